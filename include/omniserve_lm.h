@@ -11,7 +11,7 @@
 extern "C" {
 #endif
 
-#define LM_ABI_VERSION 5
+#define LM_ABI_VERSION 6
 #define LM_NORM_LAYER 0
 #define LM_NORM_RMS 1
 #define LM_EPI_ELEM 0
@@ -74,6 +74,34 @@ int lm_attn_decode(const void* qkv, int64_t ld, const void* v_first, int64_t ldv
                    const int* pos, const int* slot, void* kc, void* vc, const int* bt, int bt_stride, const void* gate, int64_t ldg,
                    void* o, int64_t ldo, float* part, int nsplit, float scale, int window, int B, int H, int G, int dk, int dv,
                    void* stream);
+
+/* ---- rotary positions, and a cache of 8-bit floats ----
+ * Both pairings: halves 0 turns (2 i, 2 i + 1), else (i, i + half); the first 2 * half dimensions of a head turn, the others stay.
+ * freq: f64, angle = position * freq[i] in 64 bits; cosine and sine times factor.  pos < 0: an empty place, nothing is done with its row. */
+/* heads of dk at column 0 of every row of x -> the same columns of o: x itself (in place), or memory that does not overlap it. */
+int lm_rope(const void* x, int64_t ldx, void* o, int64_t ldo, const double* freq, int half, const int* pos, int halves, float factor,
+            int tokens, int heads, int dk, void* stream);
+/* Pools kc [pages][G][64][dk], vc [pages][G][64][dv] of e4m3 codes, ke, ve [pages][G][64]: value = code * 2^(byte - 127), the power (from
+ * 2^-100) the least that brings the row's largest finite magnitude to 448; NaN and infinities become NaN.
+ * Rows of x: q [H][dk] k [G][dk] v [G][dv].  half > 0: keys are turned (64 bits, rounded once) and, with q, the queries into q (row stride
+ * ldq; x's own place or memory that does not overlap it).  half 0: keys as they are.  Token i is row i of x, or rows[i] (then q is null; rows
+ * outside 0 .. x_rows - 1 are none); slot[i] = page * 64 + offset, outside the pools: not stored.  No two tokens of a call have the same slot. */
+int lm_kv_store(const void* x, int64_t ldx, int x_rows, const int* rows, const double* freq, int half, const int* pos, int halves, float factor,
+                void* q, int64_t ldq, const int* slot, uint8_t* kc, uint8_t* vc, uint8_t* ke, uint8_t* ve, int64_t pages, int tokens, int H,
+                int G, int dk, int dv, void* stream);
+/* k [tokens][G][dk], v [tokens][G][dv] of the places slot[i]; zeros for a slot outside the pools. */
+int lm_kv_load(void* k, int64_t ldk, void* v, int64_t ldv, const uint8_t* kc, const uint8_t* vc, const uint8_t* ke, const uint8_t* ve,
+               int64_t pages, const int* slot, int tokens, int G, int dk, int dv, void* stream);
+/* Attention of drafted tokens: sequence b has tokens first[b] .. first[b + 1] - 1 of q [H][dk], k [G][dk], v [G][dv] (positions pos, turned
+ * already; at most max_draft, further ones are left out) and length[b] keys in the pages bt[b].  A token sees the context, and drafted token j of its sequence
+ * where bit j % 64 of mask[token][j / 64] is set, both only from position pos - window + 1 on.  It sees nothing: zeros.  Pools as above, or
+ * (ke, ve null) of elem; pages outside 0 .. pages - 1 are not seen.  part: f32 [n * H * nsplit * (dv + 2)] for nsplit > 1;
+ * lm_tree_attn_splits: how many parts suit (max_context: bound of the lengths, a hint). */
+int lm_tree_attn_splits(int B, int max_draft, int max_context, int H, int G, int dk, int dv);
+int lm_tree_attn(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const void* kc, const void* vc,
+                 const uint8_t* ke, const uint8_t* ve, int64_t pages, const int* bt, int bt_stride, int bt_width, const int* length,
+                 const int* first, const int* pos, const int64_t* mask, int words, void* o, int64_t ldo, float* part, int nsplit, float scale,
+                 int window, int B, int n, int max_draft, int H, int G, int dk, int dv, void* stream);
 
 /* Decayed linear attention; rows q [H][dk] k [H][dk] v [H][dv], `act` applied to all three.  seg [.][8]: first token, tokens,
  * slot, starts from zero, index in its entry, segments of the entry, 0, 0; all but an entry's last have seg_len tokens.

@@ -7,6 +7,7 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
+from typing import NamedTuple
 
 import torch
 
@@ -19,12 +20,16 @@ ELEM = {torch.bfloat16: "bf16", torch.float32: "f32"}
 NORM = {"layer": 0, "rms": 1}
 ACT = {None: 0, "silu": 1, "gelu_tanh": 2, "sigmoid": 3}
 EPI_ELEM, EPI_F32, EPI_GLU, EPI_GATE = 0, 1, 2, 3
-ABI = 5
+ABI = 6
 ATTN_ROWS = 128          # query rows of one prefill tile
 PAGE = 64                # tokens per cache page
 ROWS_MAX = 64            # up to here a step's products stream the weights
 NARROW = 128             # products of so few channels do for any number of rows
 CHOOSE_TOKENS = 32       # tokens of one norm_choose at most
+NO_WINDOW = 1 << 30
+CODE_SIZES = (64, 128, 256)  # head sizes of a quantised cache and of tree_attn
+PAIRING = {"neighbours": 0, "halves": 1}
+NOTHING = 27             # exponent byte of a row of zeros
 
 
 class _Part(_c.Structure):
@@ -44,6 +49,12 @@ PROTOTYPES = {
     "lm_attn_prefill_rows": (_i, [_i, _i, _i, _i]),
     "lm_attn_decode": (_i, [_vp, _i64, _vp, _i64, _f, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i64, _vp, _i64, _vp, _i, _f, _i, _i, _i,
                             _i, _i, _i, _vp]),
+    "lm_rope": (_i, [_vp, _i64, _vp, _i64, _vp, _i, _vp, _i, _f, _i, _i, _i, _vp]),
+    "lm_kv_store": (_i, [_vp, _i64, _i, _vp, _vp, _i, _vp, _i, _f, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
+    "lm_kv_load": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i, _i, _i, _i, _vp]),
+    "lm_tree_attn_splits": (_i, [_i] * 7),
+    "lm_tree_attn": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _i64, _vp, _i, _f,
+                          _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "lm_linear_prefill": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _i, _i, _vp]),
     "lm_linear_decode": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "lm_latent_append": (_i, [_vp, _i64, _i64, _vp, _f, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
@@ -84,6 +95,74 @@ def _p(t):
 
 def _ld(t):
     return 0 if t is None else t.stride(0)
+
+
+class KvCodes(NamedTuple):
+    """A layer's quantised cache: e4m3 codes [pages, kv heads, 64, size] and their rows' exponents [pages, kv heads, 64], all uint8; value =
+    code * 2^(exponent - 127).  1 / 64 .. 1 / 256 more than a byte an element."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_exp: torch.Tensor
+    v_exp: torch.Tensor
+
+
+def code_pools(pages: int, kv_heads: int, dk: int, dv: int, device) -> KvCodes:
+    """An empty quantised cache (all zeros)."""
+    codes = [torch.zeros((pages, kv_heads, PAGE, d), dtype=torch.uint8, device=device) for d in (dk, dv)]
+    return KvCodes(*codes, *(torch.full((pages, kv_heads, PAGE), NOTHING, dtype=torch.uint8, device=device) for _ in range(2)))
+
+
+def tree_masks(parents):
+    """Drafted tokens of one sequence, each with the place of its parent (-1: it follows the context; parents come first) -> (the mask words of
+    tree_attn: a token sees itself and what it descends from, [tokens, words] int64; depths [tokens] int32), on the CPU."""
+    n = len(parents)
+    words = max(1, (n + 63) // 64)
+    seen, depth = [], []
+    for i, p in enumerate(parents):
+        if not -1 <= p < i:
+            raise ValueError("token %d cannot follow token %d" % (i, p))
+        seen.append((seen[p] if p >= 0 else 0) | 1 << i)
+        depth.append(depth[p] + 1 if p >= 0 else 0)
+    signed = lambda x: x - (1 << 64) if x >> 63 else x      # noqa: E731
+    masks = [[signed(m >> 64 * w & (1 << 64) - 1) for w in range(words)] for m in seen]
+    return torch.tensor(masks, dtype=torch.int64).view(n, words), torch.tensor(depth, dtype=torch.int32)
+
+
+def _step(t):
+    """from row to row (a single row's stride may be anything)"""
+    return 0 if t is None or t.shape[0] <= 1 else t.stride(0)
+
+
+def _at16(t):
+    """rows that start at multiples of 16 bytes"""
+    return t.data_ptr() % 16 == 0 and _step(t) * t.element_size() % 16 == 0
+
+
+def _need(ok, *what):
+    if not ok:
+        raise ValueError(*what)
+
+
+def _rows(t, width, dtype, name):
+    """a matrix of at least `width` neighbouring columns"""
+    _need(t.dim() == 2 and t.shape[1] >= width and t.dtype == dtype and (t.stride(1) == 1 or t.shape[1] == 1), "%s: rows of %d or more %s" % (name, width, dtype))
+    return t
+
+
+def _index(t, n, name):
+    _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous(), "%s: %d contiguous int32" % (name, n))
+    return t
+
+
+def _pools(cache, dtype):
+    """(kv heads, key size, value size) of a quantised cache, or (dtype given) of pools of elements"""
+    k, v = cache[0], cache[1]
+    _need(len(cache) == (2 if dtype else 4), "a cache: pools of keys and values, and of their exponents where they are codes")
+    _need(k.dim() == 4 and v.dim() == 4 and k.shape[:3] == v.shape[:3] and k.shape[2] == PAGE and k.shape[3] in CODE_SIZES and v.shape[3] in CODE_SIZES,
+          "pools [pages, kv heads, %d, size], sizes %s" % (PAGE, CODE_SIZES))
+    _need(all(t.dtype == (dtype or torch.uint8) and t.is_contiguous() and t.device == k.device for t in cache), "contiguous pools of %s" % (dtype or torch.uint8))
+    _need(dtype or all(t.shape == k.shape[:3] for t in cache[2:]), "exponents [pages, kv heads, %d]" % PAGE)
+    return k.shape[1], k.shape[3], v.shape[3]
 
 
 class LmOps:
@@ -142,6 +221,103 @@ class LmOps:
         self._call("lm_attn_decode", _p(qkv), _ld(qkv), _p(v_first), _ld(v_first), lam, _p(freq), freq.numel(), _p(pos), _p(slot), _p(kc),
                    _p(vc), _p(bt), bt.stride(0), _p(gate), _ld(gate), _p(o), _ld(o), _p(part), nsplit, scale, window, qkv.shape[0], heads,
                    kv_heads, dk, dv)
+
+    # ---- rotary positions; a cache of 8-bit floats; drafted tokens ---------------------------------------------------
+    def _enqueue(self, name, tensors, *args):
+        """on the tensors' device, which all of them share"""
+        dev = tensors[0].device
+        _need(dev.type == "cuda", "tensors must live on the GPU")
+        _need(all(t is None or t.device == dev for t in tensors), "tensors of one device")
+        if dev.index == torch.cuda.current_device():
+            return self._call(name, *args)
+        with torch.cuda.device(dev):
+            self._call(name, *args)
+
+    def _turn(self, freq, pos, n, dk, pairing):
+        """arguments of a rotation"""
+        _need(pairing in PAIRING, "pairing: %s" % " or ".join(PAIRING))
+        _need((freq is None) == (pos is None), "freq and pos come together")
+        if freq is None:
+            return None, 0, None, 0
+        _need(freq.dtype == torch.float64 and freq.dim() == 1 and freq.is_contiguous() and 0 < 2 * freq.numel() <= dk, "freq: float64 of up to half of a head")
+        return _p(freq), freq.numel(), _p(_index(pos, n, "pos")), PAIRING[pairing]
+
+    def rope(self, x, freq, pos, heads, dk, *, pairing="neighbours", factor=1.0, out=None):
+        """The first 2 * len(freq) dimensions of `heads` heads of dk turned by pos * freq (float64), the cosine and sine times factor -> out:
+        x itself (in place), memory that does not overlap x, or (None) new rows [tokens, heads * dk].  Rows of a negative position are left out."""
+        n, w = x.shape[0], heads * dk
+        _need(heads > 0 and dk > 0, "heads of at least one dimension")
+        _rows(x, w, self.dtype, "x")
+        turn = self._turn(freq, pos, n, dk, pairing)
+        _need(turn[0] is not None, "rope turns by freq and pos")
+        if out is None:
+            out = torch.empty((n, w), dtype=self.dtype, device=x.device)
+        _need(_rows(out, w, self.dtype, "out").shape[0] == n, "out: as many rows as x")
+        self._enqueue("lm_rope", (x, freq, pos, out), _p(x), _step(x), _p(out), _step(out), *turn, factor, n, heads, dk)
+        return out
+
+    def kv_store(self, x, cache, slot, heads, *, freq=None, pos=None, pairing="neighbours", factor=1.0, q_out=None, rows=None):
+        """Keys and values of rows x (q [heads] k [kv heads] v [kv heads]) into a quantised cache (KvCodes) at slot = page * 64 + offset; a slot outside
+        the pools is not stored, no two tokens have the same.  freq, pos: keys are turned first, and with q_out (x's own columns, or memory that does
+        not overlap x) the queries too.  rows: token i is row rows[i] of x (of drafted tokens, those that were kept)."""
+        G, dk, dv = _pools(cache, None)
+        n = slot.shape[0] if rows is not None else x.shape[0]
+        _need(heads >= 0, "heads")
+        _rows(x, (heads + G) * dk + G * dv, self.dtype, "x")
+        _index(slot, n, "slot")
+        turn = self._turn(freq, pos, n, dk, pairing)
+        _need(q_out is None or (rows is None and heads > 0 and turn[0] is not None), "queries are turned of all rows in order")
+        _need(q_out is None or _rows(q_out, heads * dk, self.dtype, "q_out").shape[0] == n, "q_out: as many rows as x")
+        if rows is not None:
+            _index(rows, n, "rows")
+        self._enqueue("lm_kv_store", (x, *cache, slot, freq, pos, q_out, rows), _p(x), _step(x), x.shape[0], _p(rows), *turn, factor, _p(q_out), _step(q_out), _p(slot),
+                      *map(_p, cache), cache[0].shape[0], n, heads, G, dk, dv)
+
+    def kv_load(self, cache, slot, out=None):
+        """Rows (k [tokens, kv heads * dk], v [tokens, kv heads * dv]) of a quantised cache's places, zeros for a slot outside the pools; attn_prefill
+        takes 64 of them as a page."""
+        G, dk, dv = _pools(cache, None)
+        n = slot.shape[0]
+        _index(slot, n, "slot")
+        if out is None:
+            out = tuple(torch.empty((n, G * d), dtype=self.dtype, device=slot.device) for d in (dk, dv))
+        k, v = out
+        for t, d in ((k, dk), (v, dv)):
+            _need(_rows(t, G * d, self.dtype, "out").shape[0] == n and _at16(t), "out: a row per slot, at 16 bytes")
+        self._enqueue("lm_kv_load", (k, v, *cache, slot), _p(k), _step(k), _p(v), _step(v), *map(_p, cache), cache[0].shape[0], _p(slot), n, G, dk, dv)
+        return out
+
+    def tree_attn(self, q, k, v, mask, first, pos, cache, bt, length, scale, *, window=None, max_draft, max_context, out=None):
+        """Attention of drafted tokens (rows q [heads * dk], k, v [kv heads * size], turned already) over a paged cache -> [tokens, heads * dv].
+        Sequence b has the tokens first[b] .. first[b + 1] - 1, at most max_draft (further ones are left out), and length[b] cached keys in the pages
+        bt[b].  A token sees the cached keys and, of its sequence, the drafted ones whose bit is set in mask [tokens, words] (int64, tree_masks); with a
+        window only those at positions above its pos - window.  Rows that see nothing are zero; rows of no sequence stay as they are.  cache: KvCodes, or
+        (keys, values) [pages, kv heads, 64, size] of elements.  max_context: a bound of the lengths, by which the work is divided (longer ones are
+        attended to as well)."""
+        codes = len(cache) == 4
+        G, dk, dv = _pools(cache, None if codes else self.dtype)
+        n, B, H = q.shape[0], length.shape[0], q.shape[1] // dk
+        _need(H > 0 and H % G == 0 and q.shape[1] == H * dk, "q: a multiple of the %d kv heads, of %d each" % (G, dk))
+        for t, w, name in ((q, H * dk, "q"), (k, G * dk, "k"), (v, G * dv, "v")):
+            _rows(t, w, self.dtype, name)
+            _need(t.shape[0] == n and _at16(t), "%s: %d rows, at 16 bytes" % (name, n))
+        _need(mask.dtype == torch.int64 and mask.dim() == 2 and mask.shape[0] == n and mask.is_contiguous(), "mask: contiguous int64 [tokens, words]")
+        _need(0 <= max_draft <= 64 * mask.shape[1], "the mask has %d bits for %d drafted tokens" % (64 * mask.shape[1], max_draft))
+        _index(first, B + 1, "first"), _index(pos, n, "pos"), _index(length, B, "length")
+        _need(bt.dtype == torch.int32 and bt.dim() == 2 and bt.shape[0] == B and (bt.stride(1) == 1 or bt.shape[1] <= 1), "bt: int32 [sequences, pages]")
+        _need(bt.shape[1] == 0 or cache[0].shape[0] > 0, "a block table needs pages")
+        _need(scale > 0 and (window is None or window > 0), "scale and window are positive")
+        _need(max_context >= 0, "max_context is a number of keys")
+        if out is None:
+            out = torch.empty((n, H * dv), dtype=self.dtype, device=q.device)
+        _need(_rows(out, H * dv, self.dtype, "out").shape[0] == n and _step(out) % 4 == 0 and out.data_ptr() % (4 * out.element_size()) == 0, "out: a row per token, at four elements")
+        nsplit = self._h.lm_tree_attn_splits(B, max_draft, max_context, H, G, dk, dv)
+        part = torch.empty((n * H * nsplit * (dv + 2),), dtype=torch.float32, device=q.device) if nsplit > 1 else None
+        ke, ve = cache[2:] if codes else (None, None)
+        self._enqueue("lm_tree_attn", (q, k, v, *cache, bt, length, first, pos, mask, out), _p(q), _step(q), _p(k), _step(k), _p(v), _step(v), _p(cache[0]), _p(cache[1]), _p(ke), _p(ve),
+                      cache[0].shape[0], _p(bt), max(bt.stride(0), bt.shape[1]), bt.shape[1], _p(length), _p(first), _p(pos), _p(mask), mask.shape[1], _p(out), _step(out), _p(part),
+                      nsplit, scale, min(window or NO_WINDOW, NO_WINDOW), B, n, max_draft, H, G, dk, dv)
+        return out
 
     def linear_prefill(self, x, o, state, seg_state, seg, seg_len, multi, log2_decay, heads, dk, dv, act):
         self._call("lm_linear_prefill", _p(x), _ld(x), _p(o), _ld(o), _p(state), _p(seg_state), _p(seg), seg.shape[0], seg_len, int(multi),

@@ -1,0 +1,697 @@
+// Attention of drafted tokens over a paged cache: every sequence brings a few tokens (one, a chain, a tree of guesses), each of which sees
+// the cached context and, of the drafted tokens, those its mask names.
+//
+//   o = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q . k_j - max),   j over the context's keys and the drafted ones that are seen
+//
+// The drafted tokens' query heads of one kv head are rows: R = tokens * heads per kv head, 16 of them a column block of the MFMA tiles.  A
+// workgroup has NR blocks of rows of one sequence and kv head and one part of the keys; its four waves take tiles of 64 keys (32 unless the
+// cache holds codes) in turn, so that a key's codes are fetched and decoded once for all rows, and meet in LDS.  Few rows and long contexts
+// are bound by the cache's bytes, many rows by the products.
+//
+// Codes (lm_kv_codes.h).  A key's power of two scales its operand in the conversion.  A value's, 2^e, joins the softmax: with weights
+// w_j = 2^(s_j + e_j - m'), m' the running maximum of s_j + e_j, the outputs are sum w_j code_j and the sum of the probabilities is
+// sum w_j 2^(-e_j).  So w_j is at most one and is ONE f16 operand (11 bits, times 2^14 so that small ones stay normal) beside codes that f16
+// holds exactly; bf16 values need two bf16 operands for theirs (16 bits).  The drafted values, whose exponents nothing has taken out, are
+// divided by a power of two of their own.
+#include "lm_attn.h"
+#include "lm_kv_codes.h"
+#include "omniserve_lm.h"
+
+namespace lm {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+struct TreeArgs {
+  const elem_t* q; int64_t ldq;                      // [n][H][dk]
+  const elem_t* k; int64_t ldk;                      // drafted keys [n][G][dk]
+  const elem_t* v; int64_t ldv;
+  const uint8_t* kc; const uint8_t* vc;              // pools: codes, or elements
+  const uint8_t* ke; const uint8_t* ve;
+  int pages;
+  const int* bt; int bt_stride, bt_width;
+  const int* length; const int* first; const int* pos;
+  const unsigned long long* mask; int words;
+  elem_t* o; int64_t ldo;
+  float* ml; float* part;                            // nsplit > 1: [n * H][nsplit][2] and [n * H][nsplit][dv]
+  float scale;
+  int window, n, H, G, B, nsplit, max_draft, blocks;
+};
+
+// f32 of the codes' power-of-two exponents, and their reciprocals
+__device__ __forceinline__ float exponent_of(uint32_t w, int i) { return (float)(w >> (8 * i) & 255) - 127.f; }
+__device__ __forceinline__ float inverse_of(uint32_t w, int i) { return __uint_as_float((254 - (w >> (8 * i) & 255)) << 23); }
+
+template <int DK, int DV, int NR, bool CODES>
+struct Tree {
+  static constexpr bool F16 = CODES && SPLIT;                     // weights of codes are one f16 operand
+  static constexpr float SHIFT = F16 ? 14.f : 0.f;
+  static constexpr int CH = DK / 64, PF = 16 / FR, NKF = CH * PF, NVB = DV / 16;
+  static constexpr int KT = CODES ? 64 : 32, NU = KT / 16;        // keys of a context tile
+  static constexpr int STAGE = 64 * DV;                           // bytes of a wave's V tile: 64 rows of codes, 32 of bf16
+  static constexpr int RED = 4 * 16 * (DV + 4) * 4, PBUF = 4 * 4096;
+  static constexpr int LDS = (SPLIT && 4 * STAGE > RED ? 4 * STAGE : RED) > PBUF ? (SPLIT && 4 * STAGE > RED ? 4 * STAGE : RED) : PBUF;
+  typedef Tile<SPLIT ? DV * 2 : 256> VT;
+
+  const TreeArgs& p;
+  uint8_t* stage;                   // this wave's part of the LDS
+  int lane, l15, l4;
+  frag_t qf[NR][NKF];
+  f32x4 acc[NR][NVB];
+  float m_run[NR], l_run[NR];
+  int low[NR];                      // the newest position that the row does not see any more
+  bool row_ok[NR];
+
+  __device__ __forceinline__ Tree(const TreeArgs& a) : p(a) {}
+
+  // The 16-byte slot of a row of codes in LDS, so that the eight rows of both 16-lane groups of a transposed read lie in different banks.
+  __device__ __forceinline__ static int swizzle(int row) {
+    if constexpr (DV == 64) return ((row >> 2) & 1) | ((row >> 4) & 1) << 1;
+    if constexpr (DV == 128) return ((row >> 1) & 3) | ((row >> 4) & 1) << 2;
+    return (row & 7) | ((row >> 4) & 1) << 3;
+  }
+
+  __device__ __forceinline__ void wave_sync() const {      // LDS operations of one wave are in order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  // x: scores times scale plus the values' exponents, unseen ones NEG; inv: 2^-exponent.  Leaves the weights in x.
+  template <int U, bool ONE>
+  __device__ __forceinline__ void softmax(int i, f32x4 (&x)[U], const f32x4 (&inv)[U], float inv_all) {
+    float t = NEG;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t = fmaxf(t, x[u][r]);
+    t = column_max(t);
+    const float m_new = t <= NEG ? m_run[i] : fmaxf(m_run[i], t);
+    const float m_sub = (m_new <= NEG ? 0.f : m_new) - SHIFT;
+    const float alpha = __builtin_amdgcn_exp2f(m_run[i] - m_new);
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[u][r] = __builtin_amdgcn_exp2f(x[u][r] - m_sub);
+        sum = ONE ? sum + x[u][r] : __builtin_fmaf(x[u][r], inv[u][r], sum);
+      }
+    l_run[i] = l_run[i] * alpha + (ONE ? sum * inv_all : sum);
+    m_run[i] = m_new;
+    if (__any(alpha != 1.0f)) {      // (the maximum settles after a few tiles)
+#pragma unroll
+      for (int c = 0; c < NVB; ++c) acc[i][c] *= alpha;
+    }
+  }
+
+  // What non-finite values of a tile in which not every row sees every key add: they were left out of the products, where a weight of
+  // zero would have made them NaN in rows that do not see them.  w: this lane's weights, -1 where unseen.
+  template <int U, typename Value>
+  __device__ __forceinline__ void add_nonfinite(f32x4 (&a)[NVB], const f32x4 (&w)[U], Value value) {
+    float* buf = (float*)stage;
+    wave_sync();
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) buf[(16 * u + 4 * l4 + r) * 16 + l15] = w[u][r];
+    wave_sync();
+#pragma unroll 1
+    for (int j = 0; j < 16 * U; ++j) {
+      const float f = buf[16 * j + l15];
+#pragma unroll
+      for (int c = 0; c < NVB; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float y = value(j, 16 * c + 4 * l4 + r);
+          if (f >= 0.f && !(fabsf(y) < __builtin_inff())) a[c][r] += f * y;
+        }
+    }
+    wave_sync();
+  }
+
+  // ---- context tiles of codes ----
+  struct Codes {
+    u32x4 k[NU][CH], v[SPLIT ? DV / 16 : 1];
+    uint32_t kx[NU], vx[NU];
+    int64_t at;        // first row of the tile in the pools
+  };
+
+  __device__ __forceinline__ void load_codes(Codes& c, int page, int g) const {
+    c.at = ((int64_t)min(max(page, 0), p.pages - 1) * p.G + g) * PAGE;
+    const uint8_t* kp = p.kc + c.at * DK;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+#pragma unroll
+      for (int j = 0; j < CH; ++j) c.k[u][j] = *(const u32x4*)(kp + (16 * u + l15) * DK + 64 * j + 16 * l4);
+      c.kx[u] = p.ke[c.at + 16 * u + l15];
+      c.vx[u] = *(const uint32_t*)(p.ve + c.at + 16 * u + 4 * l4);
+    }
+    if constexpr (SPLIT) {
+      const uint8_t* vp = p.vc + c.at * DV;
+#pragma unroll
+      for (int i = 0; i < DV / 16; ++i) c.v[i] = *(const u32x4*)(vp + (64 * i + lane) * 16);
+    }
+  }
+
+  __device__ __forceinline__ static frag_t code_frag(const u32x4& w, int h, float scale) {
+    frag_t f;
+#pragma unroll
+    for (int m = 0; m < FR / 4; ++m) {
+      const quad_t z = decode4(w[h * (FR / 4) + m], scale);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[4 * m + e] = z[e];
+    }
+    return f;
+  }
+
+  __device__ __forceinline__ static f16x8 code_halves(u32x2 w) {
+    f16x8 f;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[m], 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[m], 1.0f, true);
+      f[4 * m] = a[0]; f[4 * m + 1] = a[1]; f[4 * m + 2] = b[0]; f[4 * m + 3] = b[1];
+    }
+    return f;
+  }
+
+  // Scores of the tile's keys, and the next tile's request behind them; keys lo .. hi - 1 of the tile exist.
+  template <typename Next>
+  __device__ __forceinline__ void code_tile(Codes& c, int kb, int lo, int hi, bool edge, Next next) {
+    f32x4 x[NR][NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) x[i][u] = zero4();
+      const float scale = scale_of(c.kx[u]);
+#pragma unroll
+      for (int j = 0; j < CH; ++j)
+#pragma unroll
+        for (int h = 0; h < PF; ++h) {
+          const frag_t kf = code_frag(c.k[u][j], h, scale);
+#pragma unroll
+          for (int i = 0; i < NR; ++i) x[i][u] = mma(kf, qf[i][j * PF + h], x[i][u]);
+        }
+    }
+    const uint8_t* vp = p.vc + c.at * DV;
+    f32x4 ev[NU], inv[NU];
+    bool bad = false;
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = 16 * u + 4 * l4 + r;
+          w |= (key >= lo && key < hi ? c.vx[u] >> (8 * r) & 255 : 127u) << (8 * r);
+        }
+        c.vx[u] = w;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) { ev[u][r] = exponent_of(c.vx[u], r); inv[u][r] = inverse_of(c.vx[u], r); }
+    if constexpr (SPLIT) {
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < DV / 16; ++i) {
+          const int row = (64 * i + lane) / (DV / 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w = row >= lo && row < hi ? c.v[i][e] : 0;
+            const uint32_t nan = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;      // bytes whose seven low bits are ones
+            bad |= nan != 0;
+            c.v[i][e] = w & ~(nan - (nan >> 7) | nan);
+          }
+        }
+        bad = __any(bad);
+      }
+      __builtin_amdgcn_wave_barrier();       // the previous tile has been read
+#pragma unroll
+      for (int i = 0; i < DV / 16; ++i) {
+        const int at = 64 * i + lane, row = at / (DV / 16), slot = at % (DV / 16);
+        *(u32x4*)(stage + row * DV + ((slot ^ swizzle(row)) << 4)) = c.v[i];
+      }
+    }
+    const int64_t here = c.at;
+    next();
+    if constexpr (SPLIT) wave_sync();
+    f16x4 pq[NR][NU];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float y = __builtin_fmaf(x[i][u][r], p.scale, ev[u][r]);
+          const int key = 16 * u + 4 * l4 + r;
+          x[i][u][r] = !edge || ((int)(key >= lo) & (int)(key < hi) & (int)(kb + key > low[i])) ? y : NEG;
+        }
+      softmax<NU, false>(i, x[i], inv, 1.f);
+      if constexpr (SPLIT) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) pq[i][u] = (f16x4){(_Float16)x[i][u][0], (_Float16)x[i][u][1], (_Float16)x[i][u][2], (_Float16)x[i][u][3]};
+      }
+    }
+    if constexpr (SPLIT) {
+      const int half_row = (l15 >> 1) < 4 ? 4 * l4 + (l15 >> 1) : 12 + 4 * l4 + (l15 >> 1);
+      const int base = half_row * DV + (swizzle(half_row) << 4) + 8 * (l15 & 1);
+      typedef int tr2 __attribute__((__vector_size__(8)));
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int cb = 0; cb < NVB; ++cb) {
+          const tr2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (__attribute__((address_space(3))) tr2*)(__attribute__((address_space(3))) void*)(stage + (base ^ (cb << 4)) + h * 32 * DV));
+          const f16x8 vf = code_halves((u32x2){(uint32_t)w[0], (uint32_t)w[1]});
+#pragma unroll
+          for (int i = 0; i < NR; ++i)
+            acc[i][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_shufflevector(pq[i][2 * h], pq[i][2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7), acc[i][cb], 0, 0, 0);
+        }
+    } else {
+#pragma unroll
+      for (int h = 0; h < NU / 2; ++h)
+#pragma unroll
+        for (int cb = 0; cb < NVB; ++cb) {
+          quad_t v[2];
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int key = 32 * h + 16 * s + 4 * l4 + r;
+              float y = decode4(vp[key * DV + 16 * cb + l15], 1.0f)[0];
+              if (edge) {
+                y = key >= lo && key < hi ? y : 0.f;
+                bad |= y != y;
+                y = y != y ? 0.f : y;
+              }
+              v[s][r] = (elem_t)y;
+            }
+#pragma unroll
+          for (int i = 0; i < NR; ++i) acc[i][cb] = mma_quads(v[0], v[1], to_quad(x[i][2 * h]), to_quad(x[i][2 * h + 1]), acc[i][cb]);
+        }
+      bad = __any(bad);
+    }
+    if (bad) {
+      const uint8_t* vb = p.vc + here * DV;
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int key = 16 * u + 4 * l4 + r;
+            if (!((int)(key >= lo) & (int)(key < hi) & (int)(kb + key > low[i]))) x[i][u][r] = -1.f;
+          }
+        add_nonfinite<NU>(acc[i], x[i], [&](int j, int d) { return j >= lo && j < hi && (vb[j * DV + d] & 127) == 127 ? __builtin_nanf("") : 0.f; });
+      }
+    }
+  }
+
+  // ---- 32 keys and values in elements: drafted ones, or a part of a page ----
+  struct Elems {
+    frag_t k[2][NKF], v[SPLIT ? DV / 16 : 1];
+    const elem_t* kp; const elem_t* vp;
+    int64_t ldk, ldv;
+    int rows;        // that exist
+  };
+
+  __device__ __forceinline__ void load_elems(Elems& c, const elem_t* kp, int64_t ldk, const elem_t* vp, int64_t ldv, int rows) const {
+    c.kp = kp; c.vp = vp; c.ldk = ldk; c.ldv = ldv; c.rows = rows;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const elem_t* row = kp + min(16 * u + l15, rows - 1) * ldk;
+#pragma unroll
+      for (int j = 0; j < CH; ++j)
+#pragma unroll
+        for (int h = 0; h < PF; ++h) c.k[u][j * PF + h] = *(const frag_t*)(row + 64 * j + 16 * l4 + FR * h);
+    }
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int i = 0; i < DV / 16; ++i) {
+        const int at = 64 * i + lane, row = at / (DV / 8), col = at % (DV / 8);
+        c.v[i] = *(const frag_t*)(vp + min(row, rows - 1) * ldv + 8 * col);
+      }
+    }
+  }
+
+  // seen(i, key): does row block i's row of this lane see key (of 32)?  lo .. hi - 1: keys that any row may see
+  template <typename Next, typename Seen>
+  __device__ __forceinline__ void elem_tile(Elems& c, int lo, int hi, bool edge, Seen seen, Next next) {
+    f32x4 x[NR][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        x[i][u] = zero4();
+#pragma unroll
+        for (int s = 0; s < NKF; ++s) x[i][u] = mma(c.k[u][s], qf[i][s], x[i][u]);
+      }
+    bool bad = false;
+    int e = 0;
+    const elem_t* vp = c.vp;
+    const int64_t ldv = c.ldv;
+    if constexpr (SPLIT) {
+      if (edge) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < DV / 16; ++i) {
+          const int row = (64 * i + lane) / (DV / 8);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            float y = row >= lo && row < hi ? (float)c.v[i][k] : 0.f;
+            const bool fine = fabsf(y) < __builtin_inff();
+            bad |= !fine;
+            y = fine ? y : 0.f;
+            top = fmaxf(top, fabsf(y));
+            c.v[i][k] = (elem_t)y;
+          }
+        }
+        bad = __any(bad);
+        if constexpr (CODES) {
+#pragma unroll
+          for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+          e = row_exponent(top);
+          const float f = pow2(-e);
+#pragma unroll
+          for (int i = 0; i < DV / 16; ++i)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) c.v[i][k] = (elem_t)((float)c.v[i][k] * f);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < DV / 16; ++i) {
+        const int at = 64 * i + lane;
+        *(frag_t*)(stage + VT::slot(at / VT::NS, at % VT::NS)) = c.v[i];
+      }
+    }
+    next();
+    if constexpr (SPLIT) wave_sync();
+    const float ev = (float)e;
+    quad_t pq[NR][2][NOPND];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float y = __builtin_fmaf(x[i][u][r], p.scale, ev);
+          x[i][u][r] = !edge || seen(i, 16 * u + 4 * l4 + r) ? y : NEG;
+        }
+      softmax<2, true>(i, x[i], x[i], pow2(-e));
+#pragma unroll
+      for (int u = 0; u < 2; ++u) split_quad(x[i][u], pq[i][u]);
+    }
+#pragma unroll
+    for (int cb = 0; cb < NVB; ++cb) {
+      quad_t v[2];
+      if constexpr (SPLIT) {
+        v[0] = VT::column_quad(stage, 0, cb, l15, l4);
+        v[1] = VT::column_quad(stage, 16, cb, l15, l4);
+      } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int key = 16 * s + 4 * l4 + r;
+            float y = (float)vp[min(key, c.rows - 1) * ldv + 16 * cb + l15];
+            if (edge) {
+              y = key >= lo && key < hi ? y : 0.f;
+              const bool fine = fabsf(y) < __builtin_inff();
+              bad |= !fine;
+              y = fine ? y : 0.f;
+            }
+            v[s][r] = (elem_t)y;
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int m = 0; m < NOPND; ++m) acc[i][cb] = mma_quads(v[0], v[1], pq[i][0][m], pq[i][1][m], acc[i][cb]);
+    }
+    if constexpr (!SPLIT) bad = __any(bad);
+    if (bad) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!seen(i, 16 * u + 4 * l4 + r)) x[i][u][r] = -1.f;
+        add_nonfinite<2>(acc[i], x[i], [&](int j, int d) { return j >= lo && j < hi ? (float)vp[j * ldv + d] : 0.f; });
+      }
+    }
+  }
+};
+
+template <int DK, int DV, int NR, bool CODES>
+__global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_attn_kernel(TreeArgs p) {
+  typedef Tree<DK, DV, NR, CODES> T;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
+  __shared__ float wm[4][16], wl[4][16];
+  const int id = xcd_contiguous(blockIdx.x, p.B * p.G * p.nsplit * p.blocks);
+  if (id < 0) return;
+  // row blocks of the same keys are neighbours: one XCD's L2 serves them
+  const int rb = id % p.blocks, split = id / p.blocks % p.nsplit, g = id / p.blocks / p.nsplit % p.G, b = id / p.blocks / p.nsplit / p.G;
+  const int f0 = min(max(p.first[b], 0), p.n), drafted = min(max(p.first[b + 1] - f0, 0), min(p.max_draft, p.n - f0));
+  const int gs = p.H / p.G, R = drafted * gs, r0 = rb * 16 * NR;
+  if (r0 >= R) return;
+  const int length = min(max(p.length[b], 0), p.bt_width * PAGE);
+  const int* bt = p.bt + (int64_t)b * p.bt_stride;
+
+  T t(p);
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  t.lane = tid & 63; t.l15 = tid & 15; t.l4 = (tid & 63) >> 4;
+  t.stage = lds + wave * (SPLIT ? T::STAGE : 4096);
+  int low_min = INT32_MAX, low_max = INT32_MIN, token[NR];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int r = r0 + 16 * i + t.l15, rc = min(r, R - 1), tk = rc / gs;
+    token[i] = f0 + tk;
+    t.row_ok[i] = r < R;
+    const int lo = p.pos[token[i]] - p.window;
+    low_min = min(low_min, lo);
+    low_max = max(low_max, lo);
+    t.low[i] = r < R ? lo : INT32_MAX;
+    const elem_t* q = p.q + (int64_t)token[i] * p.ldq + (int64_t)(g * gs + rc - tk * gs) * DK;
+#pragma unroll
+    for (int j = 0; j < T::CH; ++j)
+#pragma unroll
+      for (int h = 0; h < T::PF; ++h) t.qf[i][j * T::PF + h] = r < R ? *(const frag_t*)(q + 64 * j + 16 * t.l4 + FR * h) : frag_t{};
+#pragma unroll
+    for (int c = 0; c < T::NVB; ++c) t.acc[i][c] = zero4();
+    t.m_run[i] = NEG;
+    t.l_run[i] = 0.f;
+  }
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) {
+    low_min = min(low_min, __shfl_xor(low_min, m, 64));
+    low_max = max(low_max, __shfl_xor(low_max, m, 64));
+  }
+  low_min = __builtin_amdgcn_readfirstlane(low_min);
+  low_max = __builtin_amdgcn_readfirstlane(low_max);
+
+  // ---- the context ----
+  const int k0 = max(low_min + 1, 0), t0 = min(k0, length) / T::KT, nt = (length + T::KT - 1) / T::KT - t0;
+  const int per = (nt + p.nsplit - 1) / p.nsplit, ta = t0 + min(split * per, nt), tb = t0 + min((split + 1) * per, nt);
+  constexpr int PER_PAGE = PAGE / T::KT;
+  int tile = ta + wave;
+  if (tile < tb) {
+    int page = bt[tile / PER_PAGE];
+    if constexpr (CODES) {
+      typename T::Codes c;
+      t.load_codes(c, page, g);
+      int ahead = tile + 4 < tb ? bt[tile + 4] : 0;
+      for (; tile < tb; tile += 4) {
+        const int kb = tile * T::KT, hi = (uint32_t)page < (uint32_t)p.pages ? length - kb : 0;
+        const bool edge = hi < T::KT || kb <= low_max;
+        page = ahead;
+        t.code_tile(c, kb, max(k0 - kb, 0), hi, edge, [&]() {
+          if (tile + 4 >= tb) return;
+          t.load_codes(c, page, g);
+          ahead = tile + 8 < tb ? bt[tile + 8] : 0;
+        });
+      }
+    } else {
+      typename T::Elems c;
+      const elem_t* kc = (const elem_t*)p.kc;
+      const elem_t* vc = (const elem_t*)p.vc;
+      auto load = [&](int tl, int pg) {
+        const int64_t at = ((int64_t)min(max(pg, 0), p.pages - 1) * p.G + g) * PAGE + tl * T::KT % PAGE;
+        t.load_elems(c, kc + at * DK, DK, vc + at * DV, DV, T::KT);
+      };
+      load(tile, page);
+      int ahead = tile + 4 < tb ? bt[(tile + 4) / PER_PAGE] : 0;
+      for (; tile < tb; tile += 4) {
+        const int kb = tile * T::KT, hi = (uint32_t)page < (uint32_t)p.pages ? length - kb : 0, lo = max(k0 - kb, 0);
+        const bool edge = hi < T::KT || kb <= low_max;
+        page = ahead;
+        t.elem_tile(c, lo, hi, edge, [&](int i, int key) { return (bool)((int)(key >= lo) & (int)(key < hi) & (int)(kb + key > t.low[i])); },
+                    [&]() {
+                      if (tile + 4 >= tb) return;
+                      load(tile + 4, page);
+                      ahead = tile + 8 < tb ? bt[(tile + 8) / PER_PAGE] : 0;
+                    });
+      }
+    }
+  }
+  // ---- the drafted tokens, by the last part: waves that had a tile less come first ----
+  if (split == p.nsplit - 1) {
+    for (int j0 = 32 * ((wave - (tb - ta)) & 3); j0 < drafted; j0 += 128) {
+      typename T::Elems c;
+      const int64_t row = f0 + j0;
+      t.load_elems(c, p.k + row * p.ldk + (int64_t)g * DK, p.ldk, p.v + row * p.ldv + (int64_t)g * DV, p.ldv, min(drafted - j0, 32));
+      uint32_t bits[NR];
+      int kpos[2][4];
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+        bits[i] = t.row_ok[i] && (j0 >> 6) < p.words ? (uint32_t)(p.mask[(int64_t)token[i] * p.words + (j0 >> 6)] >> (j0 & 63)) : 0u;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) kpos[u][r] = p.pos[min((int)row + 16 * u + 4 * t.l4 + r, f0 + drafted - 1)];
+      const int hi = min(drafted - j0, 32);
+      t.elem_tile(c, 0, hi, true,
+                  [&](int i, int key) {      // (key is a constant plus 4 l4)
+                    const int u = (key - 4 * t.l4) >> 4, r = (key - 4 * t.l4) & 3;
+                    return (bool)((int)(key < hi) & (int)(bits[i] >> key & 1) & (int)(kpos[u][r] > t.low[i]));
+                  },
+                  []() {});
+    }
+  }
+
+  // ---- the waves' results ----
+  float(*res)[16][DV + 4] = (float(*)[16][DV + 4])lds;
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const float l = column_sum(t.l_run[i]);
+    __syncthreads();      // V tiles, or the block before, have been read
+#pragma unroll
+    for (int c = 0; c < T::NVB; ++c) *(f32x4*)&res[wave][t.l15][16 * c + 4 * t.l4] = t.acc[i][c];
+    if (t.l4 == 0) { wm[wave][t.l15] = t.m_run[i]; wl[wave][t.l15] = l; }
+    __syncthreads();
+    const int rows = min(16, R - r0 - 16 * i);
+    for (int at = tid; at < rows * (DV / 4); at += 256) {
+      const int rr = at / (DV / 4), d = (at - rr * (DV / 4)) * 4, r = r0 + 16 * i + rr, tk = r / gs, h = g * gs + r - tk * gs;
+      const float m = fmaxf(fmaxf(wm[0][rr], wm[1][rr]), fmaxf(wm[2][rr], wm[3][rr]));
+      f32x4 y = zero4();
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = wl[w][rr] != 0.f ? __builtin_amdgcn_exp2f(wm[w][rr] - m) : 0.f;
+        sum += f * wl[w][rr];
+        y += f * *(const f32x4*)&res[w][rr][d];
+      }
+      if (p.nsplit > 1) {
+        const int64_t at = ((int64_t)(f0 + tk) * p.H + h) * p.nsplit + split;
+        *(f32x4*)(p.part + at * DV + d) = y;
+        if (d == 0) { p.ml[2 * at] = m; p.ml[2 * at + 1] = sum; }
+      } else {
+        y *= sum != 0.f ? 1.0f / sum : 0.f;
+        *(quad_t*)(p.o + (int64_t)(f0 + tk) * p.ldo + (int64_t)h * DV + d) = to_quad(y);
+      }
+    }
+  }
+}
+
+// Joins the parts: a wave per (token, head), lane s holds the maximum and sum of part s.
+template <int DV>
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (int64_t)p.n * p.H) return;
+  const int tk = (int)(row / p.H), h = (int)(row - (int64_t)tk * p.H);
+  // rows of no sequence, or past its max_draft tokens, were not written
+  int lo = 0, hi = p.B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.first[mid] <= tk) lo = mid;
+    else hi = mid;
+  }
+  if (tk < p.first[lo] || tk >= p.first[lo + 1] || tk - p.first[lo] >= p.max_draft) return;
+  const bool in = lane < p.nsplit;
+  const float ms = in ? p.ml[2 * (row * p.nsplit + lane)] : NEG, ls = in ? p.ml[2 * (row * p.nsplit + lane) + 1] : 0.f;
+  float m = ms;
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
+  const float f = ls != 0.f ? __builtin_amdgcn_exp2f(ms - m) : 0.f, sum = wave_sum(f * ls), inv = sum != 0.f ? 1.0f / sum : 0.f;
+  const float* q = p.part + row * p.nsplit * DV;
+  float y[DV / 64] = {};
+  for (int s0 = 0; s0 < p.nsplit; s0 += 4) {
+    float v[4][DV / 64];
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int c = 0; c < DV / 64; ++c) v[s][c] = s0 + s < p.nsplit ? q[(s0 + s) * DV + 64 * c + lane] : 0.f;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const float w = s0 + s < 64 ? __shfl(f, (s0 + s) & 63, 64) : 0.f;
+#pragma unroll
+      for (int c = 0; c < DV / 64; ++c) y[c] += w != 0.f ? w * v[s][c] : 0.f;      // (an empty part's values are not written; NaN weights pass)
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < DV / 64; ++c) p.o[(int64_t)tk * p.ldo + (int64_t)h * DV + 64 * c + lane] = (elem_t)(y[c] * inv);
+}
+
+// Blocks of 16 rows of a workgroup: as many as its registers hold (f32, which no speed is asked of, takes one)
+static int row_blocks(int rows, int dk, int dv) { return rows <= 16 || !SPLIT ? 1 : rows <= 32 || dk > 128 || dv > 128 ? 2 : 4; }
+
+template <int DK, int DV, bool CODES>
+static int launch_tree(TreeArgs& a, hipStream_t s) {
+  const int rows = a.max_draft * (a.H / a.G), nr = row_blocks(rows, DK, DV);
+  a.blocks = (rows + 16 * nr - 1) / (16 * nr);
+  const int64_t groups = (int64_t)a.B * a.G * a.nsplit * a.blocks;
+  if (groups > 1 << 28) return LM_EINVAL;
+  const dim3 grid((unsigned)((groups + 7) / 8 * 8));
+  if (nr == 1) hipLaunchKernelGGL((tree_attn_kernel<DK, DV, 1, CODES>), grid, dim3(256), 0, s, a);
+  if constexpr (SPLIT) {
+    if (nr == 2) hipLaunchKernelGGL((tree_attn_kernel<DK, DV, 2, CODES>), grid, dim3(256), 0, s, a);
+    if constexpr (DK <= 128 && DV <= 128)
+      if (nr == 4) hipLaunchKernelGGL((tree_attn_kernel<DK, DV, 4, CODES>), grid, dim3(256), 0, s, a);
+  }
+  if (a.nsplit > 1) hipLaunchKernelGGL((tree_merge_kernel<DV>), dim3((unsigned)(((int64_t)a.n * a.H + 3) / 4)), dim3(256), 0, s, a);
+  return launch_status();
+}
+
+}  // namespace lm
+
+using namespace lm;
+
+// Enough workgroups for two a CU, parts of at least eight tiles
+extern "C" int lm_tree_attn_splits(int B, int max_draft, int max_context, int H, int G, int dk, int dv) {
+  if (B <= 0 || G <= 0 || H <= 0 || H % G || max_draft <= 0) return 1;
+  const int rows = max_draft * (H / G), nr = row_blocks(rows, dk, dv);
+  const int64_t groups = (int64_t)B * G * ((rows + 16 * nr - 1) / (16 * nr));
+  const int tiles = max_context / 64 + (max_context % 64 > 0);
+  const int64_t want = (512 + groups - 1) / groups;
+  return (int)max((int64_t)1, min(min(want, (int64_t)(tiles + 7) / 8), (int64_t)64));
+}
+
+extern "C" int lm_tree_attn(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const void* kc, const void* vc, const uint8_t* ke,
+                            const uint8_t* ve, int64_t pages, const int* bt, int bt_stride, int bt_width, const int* length, const int* first, const int* pos,
+                            const int64_t* mask, int words, void* o, int64_t ldo, float* part, int nsplit, float scale, int window, int B, int n, int max_draft,
+                            int H, int G, int dk, int dv, void* stream) {
+  if (B < 0 || n < 0 || max_draft < 0 || G <= 0 || H <= 0 || H % G || !(scale > 0.f) || window <= 0 || words < 0 || bt_width < 0 || bt_stride < bt_width ||
+      bt_width > INT32_MAX / PAGE || pages < 0 || pages > INT32_MAX / PAGE || (bt_width > 0 && pages == 0) || nsplit < 1 || nsplit > 64 || (nsplit > 1 && !part) ||
+      (ke == nullptr) != (ve == nullptr) || ldq % FR || ldk % FR || ldv % FR || ldo % 4 || (int64_t)max_draft * H > 1 << 24)
+    return LM_EINVAL;
+  if (B == 0 || n == 0 || max_draft == 0) return LM_OK;
+  if (!q || !k || !v || !length || !first || !pos || !mask || !o || (bt_width > 0 && (!bt || !kc || !vc)) ||
+      ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)part) % 16 || (uintptr_t)o % 8 || (uintptr_t)ve % 4)
+    return LM_EINVAL;
+  TreeArgs a{};
+  a.q = (const elem_t*)q; a.ldq = ldq; a.k = (const elem_t*)k; a.ldk = ldk; a.v = (const elem_t*)v; a.ldv = ldv;
+  a.kc = (const uint8_t*)kc; a.vc = (const uint8_t*)vc; a.ke = ke; a.ve = ve; a.pages = (int)pages;
+  a.bt = bt; a.bt_stride = bt_stride; a.bt_width = bt_width; a.length = length; a.first = first; a.pos = pos;
+  a.mask = (const unsigned long long*)mask; a.words = words; a.o = (elem_t*)o; a.ldo = ldo;
+  a.part = part; a.ml = part ? part + (int64_t)n * H * nsplit * dv : nullptr;
+  a.scale = scale * LOG2E; a.window = window; a.n = n; a.H = H; a.G = G; a.B = B; a.nsplit = nsplit; a.max_draft = max_draft;
+  hipStream_t s = (hipStream_t)stream;
+#define LM_CASE(K, V) if (dk == K && dv == V) return ke ? launch_tree<K, V, true>(a, s) : launch_tree<K, V, false>(a, s);
+  LM_CASE(64, 64) LM_CASE(64, 128) LM_CASE(64, 256) LM_CASE(128, 64) LM_CASE(128, 128) LM_CASE(128, 256)
+  LM_CASE(256, 64) LM_CASE(256, 128) LM_CASE(256, 256)
+#undef LM_CASE
+  return LM_EINVAL;
+}
