@@ -26,9 +26,6 @@ PAGE = 64                # tokens per cache page
 ROWS_MAX = 64            # up to here a step's products stream the weights
 NARROW = 128             # products of so few channels do for any number of rows
 CHOOSE_TOKENS = 32       # tokens of one norm_choose at most
-NO_WINDOW = 1 << 30
-CODE_SIZES = (64, 128, 256)  # head sizes of a quantised cache and of tree_attn
-PAIRING = {"neighbours": 0, "halves": 1}
 NOTHING = 27             # exponent byte of a row of zeros
 
 
@@ -128,41 +125,15 @@ def tree_masks(parents):
     return torch.tensor(masks, dtype=torch.int64).view(n, words), torch.tensor(depth, dtype=torch.int32)
 
 
-def _step(t):
-    """from row to row (a single row's stride may be anything)"""
-    return 0 if t is None or t.shape[0] <= 1 else t.stride(0)
-
-
-def _at16(t):
-    """rows that start at multiples of 16 bytes"""
-    return t.data_ptr() % 16 == 0 and _step(t) * t.element_size() % 16 == 0
-
-
-def _need(ok, *what):
-    if not ok:
-        raise ValueError(*what)
-
-
-def _rows(t, width, dtype, name):
-    """a matrix of at least `width` neighbouring columns"""
-    _need(t.dim() == 2 and t.shape[1] >= width and t.dtype == dtype and (t.stride(1) == 1 or t.shape[1] == 1), "%s: rows of %d or more %s" % (name, width, dtype))
-    return t
-
-
-def _index(t, n, name):
-    _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous(), "%s: %d contiguous int32" % (name, n))
-    return t
-
-
-def _pools(cache, dtype):
-    """(kv heads, key size, value size) of a quantised cache, or (dtype given) of pools of elements"""
-    k, v = cache[0], cache[1]
-    _need(len(cache) == (2 if dtype else 4), "a cache: pools of keys and values, and of their exponents where they are codes")
-    _need(k.dim() == 4 and v.dim() == 4 and k.shape[:3] == v.shape[:3] and k.shape[2] == PAGE and k.shape[3] in CODE_SIZES and v.shape[3] in CODE_SIZES,
-          "pools [pages, kv heads, %d, size], sizes %s" % (PAGE, CODE_SIZES))
-    _need(all(t.dtype == (dtype or torch.uint8) and t.is_contiguous() and t.device == k.device for t in cache), "contiguous pools of %s" % (dtype or torch.uint8))
-    _need(dtype or all(t.shape == k.shape[:3] for t in cache[2:]), "exponents [pages, kv heads, %d]" % PAGE)
-    return k.shape[1], k.shape[3], v.shape[3]
+def _binding():
+    """csrc_ext/lm_ext.cpp, built first when the checkout has none"""
+    from .. import build
+    if not os.path.exists(build.ext_path("_lm_ext")):
+        build.build_lm_ext()
+    from .. import _lm_ext
+    if _lm_ext.abi_version() != ABI:
+        raise RuntimeError("the operators' binding does not match: run `python -m omniserve_amd.build --force`")
+    return _lm_ext
 
 
 class LmOps:
@@ -182,6 +153,7 @@ class LmOps:
             raise RuntimeError("the layer library does not match its binding: run `python -m omniserve_amd.build --force`")
         self._h = h
         self.delta_chunk = h.lm_delta_chunk_rows()      # tokens per chunk of the delta rule
+        self._bound = None
 
     def _call(self, name, *args):
         _lib.check(getattr(self._h, name)(*args, _lib.current_stream()), name)
@@ -223,69 +195,29 @@ class LmOps:
                    kv_heads, dk, dv)
 
     # ---- rotary positions; a cache of 8-bit floats; drafted tokens ---------------------------------------------------
-    def _enqueue(self, name, tensors, *args):
-        """on the tensors' device, which all of them share"""
-        dev = tensors[0].device
-        _need(dev.type == "cuda", "tensors must live on the GPU")
-        _need(all(t is None or t.device == dev for t in tensors), "tensors of one device")
-        if dev.index == torch.cuda.current_device():
-            return self._call(name, *args)
-        with torch.cuda.device(dev):
-            self._call(name, *args)
-
-    def _turn(self, freq, pos, n, dk, pairing):
-        """arguments of a rotation"""
-        _need(pairing in PAIRING, "pairing: %s" % " or ".join(PAIRING))
-        _need((freq is None) == (pos is None), "freq and pos come together")
-        if freq is None:
-            return None, 0, None, 0
-        _need(freq.dtype == torch.float64 and freq.dim() == 1 and freq.is_contiguous() and 0 < 2 * freq.numel() <= dk, "freq: float64 of up to half of a head")
-        return _p(freq), freq.numel(), _p(_index(pos, n, "pos")), PAIRING[pairing]
+    # Checked and enqueued by csrc_ext/lm_ext.cpp, on the tensors' device and its current stream; a call that does not fit is a ValueError.
+    @property
+    def _x(self):
+        if self._bound is None:
+            at = lambda name: _c.cast(getattr(self._h, name), _vp).value      # noqa: E731
+            self._bound = _binding().Ops(self.dtype == torch.bfloat16, *map(at, ("lm_rope", "lm_kv_store", "lm_kv_load", "lm_tree_attn_splits", "lm_tree_attn")))
+        return self._bound
 
     def rope(self, x, freq, pos, heads, dk, *, pairing="neighbours", factor=1.0, out=None):
         """The first 2 * len(freq) dimensions of `heads` heads of dk turned by pos * freq (float64), the cosine and sine times factor -> out:
         x itself (in place), memory that does not overlap x, or (None) new rows [tokens, heads * dk].  Rows of a negative position are left out."""
-        n, w = x.shape[0], heads * dk
-        _need(heads > 0 and dk > 0, "heads of at least one dimension")
-        _rows(x, w, self.dtype, "x")
-        turn = self._turn(freq, pos, n, dk, pairing)
-        _need(turn[0] is not None, "rope turns by freq and pos")
-        if out is None:
-            out = torch.empty((n, w), dtype=self.dtype, device=x.device)
-        _need(_rows(out, w, self.dtype, "out").shape[0] == n, "out: as many rows as x")
-        self._enqueue("lm_rope", (x, freq, pos, out), _p(x), _step(x), _p(out), _step(out), *turn, factor, n, heads, dk)
-        return out
+        return self._x.rope(x, freq, pos, heads, dk, pairing, factor, out)
 
     def kv_store(self, x, cache, slot, heads, *, freq=None, pos=None, pairing="neighbours", factor=1.0, q_out=None, rows=None):
         """Keys and values of rows x (q [heads] k [kv heads] v [kv heads]) into a quantised cache (KvCodes) at slot = page * 64 + offset; a slot outside
         the pools is not stored, no two tokens have the same.  freq, pos: keys are turned first, and with q_out (x's own columns, or memory that does
         not overlap x) the queries too.  rows: token i is row rows[i] of x (of drafted tokens, those that were kept)."""
-        G, dk, dv = _pools(cache, None)
-        n = slot.shape[0] if rows is not None else x.shape[0]
-        _need(heads >= 0, "heads")
-        _rows(x, (heads + G) * dk + G * dv, self.dtype, "x")
-        _index(slot, n, "slot")
-        turn = self._turn(freq, pos, n, dk, pairing)
-        _need(q_out is None or (rows is None and heads > 0 and turn[0] is not None), "queries are turned of all rows in order")
-        _need(q_out is None or _rows(q_out, heads * dk, self.dtype, "q_out").shape[0] == n, "q_out: as many rows as x")
-        if rows is not None:
-            _index(rows, n, "rows")
-        self._enqueue("lm_kv_store", (x, *cache, slot, freq, pos, q_out, rows), _p(x), _step(x), x.shape[0], _p(rows), *turn, factor, _p(q_out), _step(q_out), _p(slot),
-                      *map(_p, cache), cache[0].shape[0], n, heads, G, dk, dv)
+        self._x.kv_store(x, cache, slot, heads, freq, pos, pairing, factor, q_out, rows)
 
     def kv_load(self, cache, slot, out=None):
         """Rows (k [tokens, kv heads * dk], v [tokens, kv heads * dv]) of a quantised cache's places, zeros for a slot outside the pools; attn_prefill
         takes 64 of them as a page."""
-        G, dk, dv = _pools(cache, None)
-        n = slot.shape[0]
-        _index(slot, n, "slot")
-        if out is None:
-            out = tuple(torch.empty((n, G * d), dtype=self.dtype, device=slot.device) for d in (dk, dv))
-        k, v = out
-        for t, d in ((k, dk), (v, dv)):
-            _need(_rows(t, G * d, self.dtype, "out").shape[0] == n and _at16(t), "out: a row per slot, at 16 bytes")
-        self._enqueue("lm_kv_load", (k, v, *cache, slot), _p(k), _step(k), _p(v), _step(v), *map(_p, cache), cache[0].shape[0], _p(slot), n, G, dk, dv)
-        return out
+        return self._x.kv_load(cache, slot, out)
 
     def tree_attn(self, q, k, v, mask, first, pos, cache, bt, length, scale, *, window=None, max_draft, max_context, out=None):
         """Attention of drafted tokens (rows q [heads * dk], k, v [kv heads * size], turned already) over a paged cache -> [tokens, heads * dv].
@@ -294,30 +226,7 @@ class LmOps:
         window only those at positions above its pos - window.  Rows that see nothing are zero; rows of no sequence stay as they are.  cache: KvCodes, or
         (keys, values) [pages, kv heads, 64, size] of elements.  max_context: a bound of the lengths, by which the work is divided (longer ones are
         attended to as well)."""
-        codes = len(cache) == 4
-        G, dk, dv = _pools(cache, None if codes else self.dtype)
-        n, B, H = q.shape[0], length.shape[0], q.shape[1] // dk
-        _need(H > 0 and H % G == 0 and q.shape[1] == H * dk, "q: a multiple of the %d kv heads, of %d each" % (G, dk))
-        for t, w, name in ((q, H * dk, "q"), (k, G * dk, "k"), (v, G * dv, "v")):
-            _rows(t, w, self.dtype, name)
-            _need(t.shape[0] == n and _at16(t), "%s: %d rows, at 16 bytes" % (name, n))
-        _need(mask.dtype == torch.int64 and mask.dim() == 2 and mask.shape[0] == n and mask.is_contiguous(), "mask: contiguous int64 [tokens, words]")
-        _need(0 <= max_draft <= 64 * mask.shape[1], "the mask has %d bits for %d drafted tokens" % (64 * mask.shape[1], max_draft))
-        _index(first, B + 1, "first"), _index(pos, n, "pos"), _index(length, B, "length")
-        _need(bt.dtype == torch.int32 and bt.dim() == 2 and bt.shape[0] == B and (bt.stride(1) == 1 or bt.shape[1] <= 1), "bt: int32 [sequences, pages]")
-        _need(bt.shape[1] == 0 or cache[0].shape[0] > 0, "a block table needs pages")
-        _need(scale > 0 and (window is None or window > 0), "scale and window are positive")
-        _need(max_context >= 0, "max_context is a number of keys")
-        if out is None:
-            out = torch.empty((n, H * dv), dtype=self.dtype, device=q.device)
-        _need(_rows(out, H * dv, self.dtype, "out").shape[0] == n and _step(out) % 4 == 0 and out.data_ptr() % (4 * out.element_size()) == 0, "out: a row per token, at four elements")
-        nsplit = self._h.lm_tree_attn_splits(B, max_draft, max_context, H, G, dk, dv)
-        part = torch.empty((n * H * nsplit * (dv + 2),), dtype=torch.float32, device=q.device) if nsplit > 1 else None
-        ke, ve = cache[2:] if codes else (None, None)
-        self._enqueue("lm_tree_attn", (q, k, v, *cache, bt, length, first, pos, mask, out), _p(q), _step(q), _p(k), _step(k), _p(v), _step(v), _p(cache[0]), _p(cache[1]), _p(ke), _p(ve),
-                      cache[0].shape[0], _p(bt), max(bt.stride(0), bt.shape[1]), bt.shape[1], _p(length), _p(first), _p(pos), _p(mask), mask.shape[1], _p(out), _step(out), _p(part),
-                      nsplit, scale, min(window or NO_WINDOW, NO_WINDOW), B, n, max_draft, H, G, dk, dv)
-        return out
+        return self._x.tree_attn(q, k, v, mask, first, pos, cache, bt, length, scale, window, max_draft, max_context, out)
 
     def linear_prefill(self, x, o, state, seg_state, seg, seg_len, multi, log2_decay, heads, dk, dv, act):
         self._call("lm_linear_prefill", _p(x), _ld(x), _p(o), _ld(o), _p(state), _p(seg_state), _p(seg), seg.shape[0], seg_len, int(multi),

@@ -9,6 +9,7 @@ go to git-ignored build/ folders beside the sources.
     libomniserve_lm_bf16.so    the layers of the serving engine's models (csrc/lm/*.hip) behind include/omniserve_lm.h,
     libomniserve_lm_f32.so     the same sources compiled for one element type each, so that a process builds and loads only
                                the one its model runs in
+    _omni_ext, _lm_ext         host-only bindings (csrc_ext/) of what is called for single tokens
 """
 from __future__ import annotations
 
@@ -63,11 +64,12 @@ def _deps_mtime(*roots) -> float:
 
 
 EXT_SRC = os.path.join(HERE, "csrc_ext", "omni_ext.cpp")
+LM_EXT_SRC = os.path.join(HERE, "csrc_ext", "lm_ext.cpp")
 
 
-def ext_path() -> str:
+def ext_path(name: str = "_omni_ext") -> str:
     import sysconfig
-    return os.path.join(HERE, "_omni_ext" + sysconfig.get_config_var("EXT_SUFFIX"))
+    return os.path.join(HERE, name + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
 def needs_build() -> bool:
@@ -77,26 +79,40 @@ def needs_build() -> bool:
     return not os.path.exists(ext) or os.path.getmtime(ext) < max(os.path.getmtime(EXT_SRC), os.path.getmtime(LIB))
 
 
-def build_ext(verbose: bool = False) -> str:
-    """The pybind11 fast path of the mirror (csrc_ext/omni_ext.cpp): host-only C++ against the installed torch's headers,
-    linked to libomniserve_hip.so next to it (rpath $ORIGIN); g++, ~25 s.  The mirror works without it (ctypes)."""
+def _build_host_ext(src: str, name: str, libs) -> str:
+    """A pybind11 module of host-only C++ against the installed torch's headers; g++, ~25 s."""
     import sysconfig
     import torch
     from torch.utils import cpp_extension as ce
-    out = ext_path()
+    out = ext_path(name)
     inc = list(ce.include_paths()) + ["/opt/rocm/include", INCLUDE, sysconfig.get_paths()["include"]]
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           "-DTORCH_EXTENSION_NAME=_omni_ext", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           "-DTORCH_EXTENSION_NAME=" + name, "-DTORCH_API_INCLUDE_EXTENSION_H",
            "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
     cmd += ["-I" + i for i in inc]
     tmp = out + ".tmp"
-    cmd += [EXT_SRC, "-o", tmp, "-L" + torch_lib, "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip", "-ltorch_hip",
-            "-L" + HERE, "-l:libomniserve_hip.so", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + torch_lib]
+    cmd += [src, "-o", tmp, "-L" + torch_lib, "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip", "-ltorch_hip", *libs,
+            "-Wl,-rpath," + torch_lib]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError("building the pybind11 fast path failed:\n%s" % r.stderr[-4000:])
+        raise RuntimeError("building %s failed:\n%s" % (name, r.stderr[-4000:]))
     os.replace(tmp, out)
+    return out
+
+
+def build_ext(verbose: bool = False) -> str:
+    """The pybind11 fast path of the mirror (csrc_ext/omni_ext.cpp), linked to libomniserve_hip.so next to it (rpath $ORIGIN).
+    The mirror works without it (ctypes)."""
+    return _build_host_ext(EXT_SRC, "_omni_ext", ["-L" + HERE, "-l:libomniserve_hip.so", "-Wl,-rpath,$ORIGIN"])
+
+
+def build_lm_ext(force: bool = False) -> str:
+    """The binding of the engine's operators for drafted tokens and the quantised cache (csrc_ext/lm_ext.cpp); the layer libraries are handed to it."""
+    out = ext_path("_lm_ext")
+    with _build_lock():
+        if force or not os.path.exists(out) or os.path.getmtime(out) < max(os.path.getmtime(LM_EXT_SRC), os.path.getmtime(os.path.join(INCLUDE, "omniserve_lm.h"))):
+            _build_host_ext(LM_EXT_SRC, "_lm_ext", [])
     return out
 
 
@@ -166,7 +182,7 @@ def build_lm(elem: str, force: bool = False, verbose: bool = False) -> str:
 
 
 def build_all(force: bool = False, verbose: bool = False) -> list:
-    return [build(force, verbose)] + [build_lm(e, force, verbose) for e in LM_ELEM]
+    return [build(force, verbose)] + [build_lm(e, force, verbose) for e in LM_ELEM] + [build_lm_ext(force)]
 
 
 if __name__ == "__main__":
