@@ -13,30 +13,10 @@
 // sum w_j 2^(-e_j).  So w_j is at most one and is ONE f16 operand (11 bits, times 2^14 so that small ones stay normal) beside codes that f16
 // holds exactly; bf16 values need two bf16 operands for theirs (16 bits).  The drafted values, whose exponents nothing has taken out, are
 // divided by a power of two of their own.
-#include "lm_attn.h"
-#include "lm_kv_codes.h"
+#include "lm_tree.h"
 #include "omniserve_lm.h"
 
 namespace lm {
-
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-
-struct TreeArgs {
-  const elem_t* q; int64_t ldq;                      // [n][H][dk]
-  const elem_t* k; int64_t ldk;                      // drafted keys [n][G][dk]
-  const elem_t* v; int64_t ldv;
-  const uint8_t* kc; const uint8_t* vc;              // pools: codes, or elements
-  const uint8_t* ke; const uint8_t* ve;
-  int pages;
-  const int* bt; int bt_stride, bt_width;
-  const int* length; const int* first; const int* pos;
-  const unsigned long long* mask; int words;
-  elem_t* o; int64_t ldo;
-  float* ml; float* part;                            // nsplit > 1: [n * H][nsplit][2] and [n * H][nsplit][dv]
-  float scale;
-  int window, n, H, G, B, nsplit, max_draft, blocks;
-};
 
 // f32 of the codes' power-of-two exponents, and their reciprocals
 __device__ __forceinline__ float exponent_of(uint32_t w, int i) { return (float)(w >> (8 * i) & 255) - 127.f; }
@@ -63,13 +43,6 @@ struct Tree {
   bool row_ok[NR];
 
   __device__ __forceinline__ Tree(const TreeArgs& a) : p(a) {}
-
-  // The 16-byte slot of a row of codes in LDS, so that the eight rows of both 16-lane groups of a transposed read lie in different banks.
-  __device__ __forceinline__ static int swizzle(int row) {
-    if constexpr (DV == 64) return ((row >> 2) & 1) | ((row >> 4) & 1) << 1;
-    if constexpr (DV == 128) return ((row >> 1) & 3) | ((row >> 4) & 1) << 2;
-    return (row & 7) | ((row >> 4) & 1) << 3;
-  }
 
   __device__ __forceinline__ void wave_sync() const {      // LDS operations of one wave are in order
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -164,16 +137,6 @@ struct Tree {
     return f;
   }
 
-  __device__ __forceinline__ static f16x8 code_halves(u32x2 w) {
-    f16x8 f;
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[m], 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[m], 1.0f, true);
-      f[4 * m] = a[0]; f[4 * m + 1] = a[1]; f[4 * m + 2] = b[0]; f[4 * m + 3] = b[1];
-    }
-    return f;
-  }
-
   // Scores of the tile's keys, and the next tile's request behind them; keys lo .. hi - 1 of the tile exist.
   template <typename Next>
   __device__ __forceinline__ void code_tile(Codes& c, int kb, int lo, int hi, bool edge, Next next) {
@@ -218,10 +181,7 @@ struct Tree {
           const int row = (64 * i + lane) / (DV / 16);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            uint32_t w = row >= lo && row < hi ? c.v[i][e] : 0;
-            const uint32_t nan = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;      // bytes whose seven low bits are ones
-            bad |= nan != 0;
-            c.v[i][e] = w & ~(nan - (nan >> 7) | nan);
+            c.v[i][e] = row >= lo && row < hi ? drop_nan_codes(c.v[i][e], bad) : 0u;
           }
         }
         bad = __any(bad);
@@ -230,7 +190,7 @@ struct Tree {
 #pragma unroll
       for (int i = 0; i < DV / 16; ++i) {
         const int at = 64 * i + lane, row = at / (DV / 16), slot = at % (DV / 16);
-        *(u32x4*)(stage + row * DV + ((slot ^ swizzle(row)) << 4)) = c.v[i];
+        *(u32x4*)(stage + row * DV + ((slot ^ code_swizzle<DV>(row)) << 4)) = c.v[i];
       }
     }
     const int64_t here = c.at;
@@ -254,16 +214,12 @@ struct Tree {
       }
     }
     if constexpr (SPLIT) {
-      const int half_row = (l15 >> 1) < 4 ? 4 * l4 + (l15 >> 1) : 12 + 4 * l4 + (l15 >> 1);
-      const int base = half_row * DV + (swizzle(half_row) << 4) + 8 * (l15 & 1);
-      typedef int tr2 __attribute__((__vector_size__(8)));
+      const int base = code_column<DV>(l15, l4);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int cb = 0; cb < NVB; ++cb) {
-          const tr2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-              (__attribute__((address_space(3))) tr2*)(__attribute__((address_space(3))) void*)(stage + (base ^ (cb << 4)) + h * 32 * DV));
-          const f16x8 vf = code_halves((u32x2){(uint32_t)w[0], (uint32_t)w[1]});
+          const f16x8 vf = code_halves(read_code_column<DV>(stage, base, h, cb));
 #pragma unroll
           for (int i = 0; i < NR; ++i)
             acc[i][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_shufflevector(pq[i][2 * h], pq[i][2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7), acc[i][cb], 0, 0, 0);
@@ -450,15 +406,10 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
   typedef Tree<DK, DV, NR, CODES> T;
   __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
   __shared__ float wm[4][16], wl[4][16];
-  const int id = xcd_contiguous(blockIdx.x, p.B * p.G * p.nsplit * p.blocks);
-  if (id < 0) return;
-  // row blocks of the same keys are neighbours: one XCD's L2 serves them
-  const int rb = id % p.blocks, split = id / p.blocks % p.nsplit, g = id / p.blocks / p.nsplit % p.G, b = id / p.blocks / p.nsplit / p.G;
-  const int f0 = min(max(p.first[b], 0), p.n), drafted = min(max(p.first[b + 1] - f0, 0), min(p.max_draft, p.n - f0));
-  const int gs = p.H / p.G, R = drafted * gs, r0 = rb * 16 * NR;
-  if (r0 >= R) return;
-  const int length = min(max(p.length[b], 0), p.bt_width * PAGE);
-  const int* bt = p.bt + (int64_t)b * p.bt_stride;
+  Share sh;
+  if (!share_of(p, sh, 16 * NR)) return;
+  const int split = sh.split, g = sh.g, f0 = sh.f0, drafted = sh.drafted, gs = sh.gs, R = sh.R, r0 = sh.rb * 16 * NR, length = sh.length;
+  const int* bt = sh.bt;
 
   T t(p);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -635,37 +586,42 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p) {
   for (int c = 0; c < DV / 64; ++c) p.o[(int64_t)tk * p.ldo + (int64_t)h * DV + 64 * c + lane] = (elem_t)(y[c] * inv);
 }
 
-// Blocks of 16 rows of a workgroup: as many as its registers hold (f32, which no speed is asked of, takes one)
-static int row_blocks(int rows, int dk, int dv) { return rows <= 16 || !SPLIT ? 1 : rows <= 32 || dk > 128 || dv > 128 ? 2 : 4; }
+// Blocks of 16 rows of a workgroup
+static int row_blocks(int rows) { return rows <= 16 || !SPLIT ? 1 : 2; }
 
 template <int DK, int DV, bool CODES>
 static int launch_tree(TreeArgs& a, hipStream_t s) {
-  const int rows = a.max_draft * (a.H / a.G), nr = row_blocks(rows, DK, DV);
+  const int rows = a.max_draft * (a.H / a.G), nr = row_blocks(rows);
   a.blocks = (rows + 16 * nr - 1) / (16 * nr);
   const int64_t groups = (int64_t)a.B * a.G * a.nsplit * a.blocks;
   if (groups > 1 << 28) return LM_EINVAL;
   const dim3 grid((unsigned)((groups + 7) / 8 * 8));
   if (nr == 1) hipLaunchKernelGGL((tree_attn_kernel<DK, DV, 1, CODES>), grid, dim3(256), 0, s, a);
-  if constexpr (SPLIT) {
+  if constexpr (SPLIT && DV <= 128)
     if (nr == 2) hipLaunchKernelGGL((tree_attn_kernel<DK, DV, 2, CODES>), grid, dim3(256), 0, s, a);
-    if constexpr (DK <= 128 && DV <= 128)
-      if (nr == 4) hipLaunchKernelGGL((tree_attn_kernel<DK, DV, 4, CODES>), grid, dim3(256), 0, s, a);
-  }
-  if (a.nsplit > 1) hipLaunchKernelGGL((tree_merge_kernel<DV>), dim3((unsigned)(((int64_t)a.n * a.H + 3) / 4)), dim3(256), 0, s, a);
   return launch_status();
+}
+
+static void launch_merge(const TreeArgs& a, int dv, hipStream_t s) {
+  const dim3 grid((unsigned)(((int64_t)a.n * a.H + 3) / 4));
+  if (dv == 64) hipLaunchKernelGGL((tree_merge_kernel<64>), grid, dim3(256), 0, s, a);
+  else if (dv == 128) hipLaunchKernelGGL((tree_merge_kernel<128>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((tree_merge_kernel<256>), grid, dim3(256), 0, s, a);
 }
 
 }  // namespace lm
 
 using namespace lm;
 
-// Enough workgroups for two a CU, parts of at least eight tiles
+// Enough workgroups for two waves a SIMD, parts of at least eight tiles
 extern "C" int lm_tree_attn_splits(int B, int max_draft, int max_context, int H, int G, int dk, int dv) {
   if (B <= 0 || G <= 0 || H <= 0 || H % G || max_draft <= 0) return 1;
-  const int rows = max_draft * (H / G), nr = row_blocks(rows, dk, dv);
-  const int64_t groups = (int64_t)B * G * ((rows + 16 * nr - 1) / (16 * nr));
+  const int rows = max_draft * (H / G);
+  const bool wide = tree_wide_takes(rows, dk, dv);
+  const int each = wide ? tree_wide_rows(rows, dk, dv) : 16 * row_blocks(rows);
+  const int64_t groups = (int64_t)B * G * ((rows + each - 1) / each), fill = wide ? 256 * 256 / each : 512;
   const int tiles = max_context / 64 + (max_context % 64 > 0);
-  const int64_t want = (512 + groups - 1) / groups;
+  const int64_t want = (fill + groups - 1) / groups;
   return (int)max((int64_t)1, min(min(want, (int64_t)(tiles + 7) / 8), (int64_t)64));
 }
 
@@ -689,9 +645,13 @@ extern "C" int lm_tree_attn(const void* q, int64_t ldq, const void* k, int64_t l
   a.part = part; a.ml = part ? part + (int64_t)n * H * nsplit * dv : nullptr;
   a.scale = scale * LOG2E; a.window = window; a.n = n; a.H = H; a.G = G; a.B = B; a.nsplit = nsplit; a.max_draft = max_draft;
   hipStream_t s = (hipStream_t)stream;
-#define LM_CASE(K, V) if (dk == K && dv == V) return ke ? launch_tree<K, V, true>(a, s) : launch_tree<K, V, false>(a, s);
+  int rc = LM_EINVAL;
+  if (tree_wide_takes(max_draft * (H / G), dk, dv)) rc = launch_tree_wide(a, dk, dv, s);
+#define LM_CASE(K, V) else if (dk == K && dv == V) rc = ke ? launch_tree<K, V, true>(a, s) : launch_tree<K, V, false>(a, s);
   LM_CASE(64, 64) LM_CASE(64, 128) LM_CASE(64, 256) LM_CASE(128, 64) LM_CASE(128, 128) LM_CASE(128, 256)
   LM_CASE(256, 64) LM_CASE(256, 128) LM_CASE(256, 256)
 #undef LM_CASE
-  return LM_EINVAL;
+  if (rc != LM_OK) return rc;
+  if (nsplit > 1) launch_merge(a, dv, s);
+  return launch_status();
 }

@@ -1,0 +1,540 @@
+// Attention of drafted tokens, many rows (tokens * heads per kv head): the waves of a workgroup have 16 or 32 rows each and share a ring of key and
+// value tiles that DMA fills two tiles ahead.  See lm_tree_attn.hip for the formula; here a tile is 64 keys of codes, or 32 of elements.
+//
+// Bound by the vector units beside the matrix units (a softmax weight costs 4 vector instructions, one of them an exponential of four times the
+// length, and 256 operations of the matrix units), so that what a weight does not need is done elsewhere:
+//   keys stay codes: the scaled MFMA takes them with their power of two.  A query row becomes TWO rows of codes, q = 2^e (hi + lo / 16): an element's
+//     8 significant bits are 4 and 4, and what is smaller than 2^-15 of the row's largest is off by at most 2^-21 of that.  Two products of 128 at
+//     twice the rate of bf16: as long as one, and no conversion;
+//   a value's exponent (lm_tree_attn.hip) is the products' initial accumulator, e / scale;
+//   2^-e and e / scale are formed by one lane per key and read back from LDS.
+#include "lm_tree.h"
+
+namespace lm {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
+#if LM_ELEM == 0
+// The 16-byte slot of a row of dk bytes that the fragments of 16 rows are read from
+template <int ROWB>
+__device__ __forceinline__ int key_swizzle(int row) {
+  if constexpr (ROWB == 64) return (4 - (row >> 2 & 3)) & 3;
+  else return Tile<ROWB>::swizzle(row);
+}
+
+template <int DK, int DV, int NW, bool CODES>
+struct Wide {
+  static constexpr int NR = DV > 128 ? 1 : 2, ROWS = NW * 16 * NR, NVB = DV / 16;
+  static constexpr int KT = CODES ? 64 : 32, NU = KT / 16;
+  static constexpr int KB = CODES ? DK : 2 * DK, VB = CODES ? DV : 2 * DV;      // bytes of a row
+  static constexpr int KBYTES = KT * KB, VBYTES = KT * VB, EXPS = CODES ? 128 : 0;
+  static constexpr int SLOT = KBYTES + VBYTES + EXPS;                            // of the ring
+  static constexpr int NBUF = NW == 2 ? 2 : 3;
+  static constexpr int KP = KBYTES / 1024, VP = VBYTES / 1024, EACH = (KP + VP + NW - 1) / NW, PIECES = EACH + (CODES ? 1 : 0);      // of a wave
+  static constexpr int OWN = 4096;                                               // a wave's: exponents; weights of a tile with non-finite values
+  static constexpr int LDS = NBUF * SLOT + NW * OWN + 64;
+  static constexpr int KS = CODES ? (DK + 127) / 128 : DK / 32;                  // steps of a key's product
+  static constexpr float SHIFT = CODES ? 14.f : 0.f;
+  typedef Tile<2 * DV> VT;
+  typedef Tile<2 * DK> KTile;
+};
+
+template <int DK, int DV, int NW, bool CODES>
+__global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
+  typedef Wide<DK, DV, NW, CODES> W;
+  constexpr int NR = W::NR, NU = W::NU, NVB = W::NVB, KT = W::KT;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  Share s;
+  if (!share_of(p, s, W::ROWS)) return;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l15 = lane & 15, l4 = lane >> 4;
+  uint8_t* own = lds + W::NBUF * W::SLOT + wave * W::OWN;
+  int* shared = (int*)(lds + W::NBUF * W::SLOT + NW * W::OWN);      // smallest, largest of the rows' bounds; a tile's largest value, whether it has non-finite ones
+  const int r0 = s.rb * W::ROWS + wave * 16 * NR;
+  const bool live = r0 < s.R;                                         // (a wave without rows fetches its pieces and waits with the others)
+
+  // ---- rows ----
+  int low[NR], token[NR], low_min = INT32_MAX, low_max = INT32_MIN;
+  bool row_ok[NR];
+  const elem_t* qrow[NR];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int r = r0 + 16 * i + l15, rc = min(r, s.R - 1), tk = rc / s.gs;
+    token[i] = s.f0 + tk;
+    row_ok[i] = r < s.R;
+    const int lo = p.pos[token[i]] - p.window;
+    low_min = min(low_min, lo);
+    low_max = max(low_max, lo);
+    low[i] = r < s.R ? lo : INT32_MAX;
+    qrow[i] = p.q + (int64_t)token[i] * p.ldq + (int64_t)(s.g * s.gs + rc - tk * s.gs) * DK;
+  }
+  if (tid == 0) { shared[0] = INT32_MAX; shared[1] = INT32_MIN; }
+  __syncthreads();
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) {
+    low_min = min(low_min, __shfl_xor(low_min, m, 64));
+    low_max = max(low_max, __shfl_xor(low_max, m, 64));
+  }
+  if (lane == 0) { atomicMin(&shared[0], low_min); atomicMax(&shared[1], low_max); }
+  __syncthreads();
+  low_min = __builtin_amdgcn_readfirstlane(shared[0]);
+  low_max = __builtin_amdgcn_readfirstlane(shared[1]);
+  const int k0 = max(low_min + 1, 0), t0 = min(k0, s.length) / KT, nt = (s.length + KT - 1) / KT - t0;
+  const int per = (nt + p.nsplit - 1) / p.nsplit, ta = t0 + min(s.split * per, nt), tb = t0 + min((s.split + 1) * per, nt);
+
+  // ---- the ring ----
+  // Offsets of this lane's pieces: place in the slot -> byte of the tile in memory
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  auto piece_of = [&](int j) { return min(j * NW + wave, W::KP + W::VP - 1); };      // (the last piece twice where they do not divide: equal bytes)
+  int from[W::EACH];
+#pragma unroll
+  for (int j = 0; j < W::EACH; ++j) {
+    const int pc = piece_of(j), key = pc < W::KP, at = (key ? pc : pc - W::KP) * 1024 + lane * 16, rowb = key ? W::KB : W::VB, row = at / rowb;
+    const int swz = key ? (CODES ? key_swizzle<W::KB>(row) : W::KTile::swizzle(row)) : (CODES ? code_swizzle<DV>(row) : W::VT::swizzle(row));
+    from[j] = row * rowb + (((at % rowb >> 4) ^ swz) << 4);
+  }
+  auto fetch = [&](int t, int page, int slot) {
+    const int64_t at = ((int64_t)min(max(page, 0), p.pages - 1) * p.G + s.g) * PAGE + (CODES ? 0 : t * KT % PAGE);
+    const uint32_t to = lds0 + slot * W::SLOT;
+#pragma unroll
+    for (int j = 0; j < W::EACH; ++j) {
+      const int pc = piece_of(j);
+      dma16_uncounted((pc < W::KP ? p.kc + at * W::KB : p.vc + at * W::VB) + from[j], to + pc * 1024);
+    }
+    if constexpr (CODES)      // (every wave, so that all have as many pieces in flight: the same bytes to the same place)
+      if (lane < 8) dma16_uncounted((lane < 4 ? p.ke : p.ve) + at + 16 * (lane & 3), to + W::KBYTES + W::VBYTES);
+  };
+  constexpr int PER_PAGE = PAGE / KT;
+  // (scalar loads: a vector load's wait would take in the DMA behind it)
+  const __attribute__((address_space(4))) int* bt = (const __attribute__((address_space(4))) int*)(uintptr_t)s.bt;
+  auto page_of = [&](int t) { return t < tb ? bt[t / PER_PAGE] : 0; };
+  int pages[W::NBUF];      // of tiles t, t + 1, ..
+#pragma unroll
+  for (int j = 0; j < W::NBUF; ++j) pages[j] = page_of(ta + j);
+#pragma unroll
+  for (int j = 0; j < W::NBUF - 1; ++j)
+    if (ta + j < tb) fetch(ta + j, pages[j], j);
+
+  // ---- queries ----
+  i32x8 qc[NR][2][CODES ? W::KS : 1];      // codes: hi, lo
+  int qe[NR][2];                           // their exponent bytes
+  frag_t qf[NR][CODES ? 1 : W::KS];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    if constexpr (CODES) {
+      float y[W::KS][32], top = 0.f;
+#pragma unroll
+      for (int k = 0; k < W::KS; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const frag_t f = row_ok[i] && 128 * k + 64 * j < DK ? *(const frag_t*)(qrow[i] + 128 * k + 64 * j + 16 * l4 + 8 * h) : frag_t{};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              y[k][16 * j + 8 * h + e] = (float)f[e];
+              const float m = fabsf((float)f[e]);
+              top = m < __builtin_inff() ? fmaxf(top, m) : top;
+            }
+          }
+      const int e = row_exponent(column_max(top));
+      qe[i][0] = e + 127;
+      qe[i][1] = e + 123;
+#pragma unroll
+      for (int k = 0; k < W::KS; ++k)
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+          const uint32_t hi = encode4(&y[k][4 * w], e);
+          const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, 1.0f, true);
+          const float f = pow2(-e), back[4] = {a[0], a[1], b[0], b[1]};
+          float rest[4];
+#pragma unroll
+          for (int m = 0; m < 4; ++m) rest[m] = 16.f * (y[k][4 * w + m] * f - back[m]);
+          qc[i][0][k][w] = (int)hi;
+          qc[i][1][k][w] = (int)encode4(rest, 0);
+        }
+    } else {
+#pragma unroll
+      for (int k = 0; k < W::KS; ++k) qf[i][k] = row_ok[i] ? *(const frag_t*)(qrow[i] + 32 * k + 8 * l4) : frag_t{};
+    }
+  }
+
+  f32x4 acc[NR][NVB];
+  float m_run[NR], l_run[NR];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+#pragma unroll
+    for (int c = 0; c < NVB; ++c) acc[i][c] = zero4();
+    m_run[i] = NEG;
+    l_run[i] = 0.f;
+  }
+  const float inv_scale = 1.0f / p.scale;
+
+  // x: scores (with e / scale), unseen ones NEG -> weights
+  auto softmax = [&](int i, auto& x, const auto& inv, auto one, float inv_all) {
+    constexpr int U = sizeof(x) / sizeof(f32x4);
+    float t = NEG;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t = fmaxf(t, x[u][r]);
+    t = column_max(t);
+    const float m_new = t <= NEG ? m_run[i] : fmaxf(m_run[i], t * p.scale);
+    const float m_sub = (m_new <= NEG ? 0.f : m_new) - W::SHIFT;
+    const float alpha = __builtin_amdgcn_exp2f(m_run[i] - m_new);
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][r], p.scale, -m_sub));
+        if constexpr (one.value) sum += x[u][r];
+        else sum = __builtin_fmaf(x[u][r], inv[u][r], sum);
+      }
+    l_run[i] = __builtin_fmaf(l_run[i], alpha, one.value ? sum * inv_all : sum);
+    m_run[i] = m_new;
+    if (__any(alpha != 1.0f)) {
+#pragma unroll
+      for (int c = 0; c < NVB; ++c) acc[i][c] *= alpha;
+    }
+  };
+  auto wave_sync = [&]() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  // What a tile's non-finite values add (lm_tree_attn.hip): x: weights, -1 where unseen
+  auto add_nonfinite = [&](int i, const auto& x, auto value) {
+    constexpr int U = sizeof(x) / sizeof(f32x4);
+    float* buf = (float*)own;
+    wave_sync();
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) buf[(16 * u + 4 * l4 + r) * 16 + l15] = x[u][r];
+    wave_sync();
+#pragma unroll 1
+    for (int j = 0; j < 16 * U; ++j) {
+      const float f = buf[16 * j + l15];
+#pragma unroll
+      for (int c = 0; c < NVB; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float y = value(j, 16 * c + 4 * l4 + r);
+          if (f >= 0.f && !(fabsf(y) < __builtin_inff())) acc[i][c][r] += f * y;
+        }
+    }
+    wave_sync();
+  };
+  // A tile of 32 keys and values in elements at `tile`: products, weights, products
+  auto elem_products = [&](const uint8_t* kt, const uint8_t* vt, const frag_t (&q)[NR][DK / 32], bool edge, bool bad, int e, auto seen, auto value) {
+    f32x4 x[NR][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int k = 0; k < DK / 32; ++k) {
+        const frag_t kf = W::KTile::frag(kt, 16 * u + l15, 4 * k + l4);
+#pragma unroll
+        for (int i = 0; i < NR; ++i) x[i][u] = mma(kf, q[i][k], k == 0 ? (f32x4)((float)e * inv_scale) : x[i][u]);
+      }
+    quad_t pq[NR][2][2];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      if (edge) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, 16 * u + 4 * l4 + r) ? x[i][u][r] : NEG;
+      }
+      softmax(i, x[i], x[i], Yes(), pow2(-e));
+#pragma unroll
+      for (int u = 0; u < 2; ++u) split_quad(x[i][u], pq[i][u]);
+    }
+#pragma unroll
+    for (int c = 0; c < NVB; ++c) {
+      const quad_t v0 = W::VT::column_quad(vt, 0, c, l15, l4), v1 = W::VT::column_quad(vt, 16, c, l15, l4);
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) acc[i][c] = mma_quads(v0, v1, pq[i][0][m], pq[i][1][m], acc[i][c]);
+    }
+    if (bad) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!seen(i, 16 * u + 4 * l4 + r)) x[i][u][r] = -1.f;
+        add_nonfinite(i, x[i], value);
+      }
+    }
+  };
+  // Values of a tile that not every row sees: rows outside lo .. hi - 1 and non-finite ones become zero; elements are divided by 2^e (codes' kernel).
+  // -> whether there were non-finite ones
+  auto clean_elems = [&](uint8_t* vt, int lo, int hi, int& e) {
+    if (tid == 0) { shared[2] = 0; shared[3] = 0; }
+    __syncthreads();
+    bool bad = false;
+    float top = 0.f;
+    for (int i = tid; i < 32 * DV / 8; i += 64 * NW) {
+      const int row = i / (DV / 8);
+      frag_t* at = (frag_t*)(vt + W::VT::slot(row, i % (DV / 8)));
+      frag_t f = *at;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float y = row >= lo && row < hi ? (float)f[k] : 0.f;
+        const bool fine = fabsf(y) < __builtin_inff();
+        bad |= !fine;
+        y = fine ? y : 0.f;
+        top = fmaxf(top, fabsf(y));
+        f[k] = (elem_t)y;
+      }
+      *at = f;
+    }
+    if (bad) atomicOr(&shared[2], 1);
+    atomicMax(&shared[3], (int)__float_as_uint(top));      // (not negative: ordered like whole numbers)
+    __syncthreads();
+    bad = shared[2] != 0;
+    e = 0;
+    if constexpr (CODES) {
+      e = row_exponent(__uint_as_float((uint32_t)shared[3]));
+      const float f = pow2(-e);
+      for (int i = tid; i < 32 * DV / 8; i += 64 * NW) {
+        frag_t* at = (frag_t*)(vt + W::VT::slot(i / (DV / 8), i % (DV / 8)));
+        frag_t y = *at;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = (elem_t)((float)y[k] * f);
+        *at = y;
+      }
+      __syncthreads();
+    }
+    return bad;
+  };
+
+  // ---- the context ----
+  int slot = 0;
+  for (int t = ta; t < tb; ++t) {
+    const int kb = t * KT, page = pages[0], hi = (uint32_t)page < (uint32_t)p.pages ? s.length - kb : 0, lo = max(k0 - kb, 0);
+    const bool edge = hi < KT || kb <= low_max;
+    if (W::NBUF > 2 && t + 1 < tb) wait_pieces<W::PIECES>();
+    else wait_pieces<0>();
+    __syncthreads();      // tile t is there; everyone has read the one before it
+    if (t + W::NBUF - 1 < tb) fetch(t + W::NBUF - 1, pages[W::NBUF - 1], slot + W::NBUF - 1 >= W::NBUF ? slot - 1 : slot + W::NBUF - 1);
+#pragma unroll
+    for (int j = 0; j + 1 < W::NBUF; ++j) pages[j] = pages[j + 1];
+    pages[W::NBUF - 1] = page_of(t + W::NBUF);
+    uint8_t* kt = lds + slot * W::SLOT;
+    uint8_t* vt = kt + W::KBYTES;
+    slot = slot + 1 == W::NBUF ? 0 : slot + 1;
+    const int64_t at = ((int64_t)min(max(page, 0), p.pages - 1) * p.G + s.g) * PAGE + (CODES ? 0 : kb % PAGE);
+    auto seen = [&](int i, int key) { return (bool)((int)(key >= lo) & (int)(key < hi) & (int)(kb + key > low[i])); };
+    bool bad = false;
+    if constexpr (!CODES) {
+      if (edge) {
+        int e;
+        bad = clean_elems(vt, lo, hi, e);
+      }
+      if (live) {
+        const elem_t* vb = (const elem_t*)p.vc + at * DV;
+        elem_products(kt, vt, qf, edge, bad, 0, seen, [&](int j, int d) { return j >= lo && j < hi ? (float)vb[j * DV + d] : 0.f; });
+      }
+    } else {
+      uint8_t* exps = vt + W::VBYTES;
+      if (edge) {
+        if (tid == 0) shared[2] = 0;
+        __syncthreads();
+        for (int i = tid; i < KT * DV / 16; i += 64 * NW) {
+          const int row = i / (DV / 16);
+          u32x4* to = (u32x4*)(vt + row * DV + (i % (DV / 16)) * 16);      // (a row's slots in any order)
+          u32x4 w = *to;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = row >= lo && row < hi ? drop_nan_codes(w[k], bad) : 0u;
+          *to = w;
+        }
+        if (tid < KT && !(tid >= lo && tid < hi)) exps[64 + tid] = 127;
+        if (bad) atomicOr(&shared[2], 1);
+        __syncthreads();
+        bad = shared[2] != 0;
+      }
+      if (live) {
+        f32x4* mine = (f32x4*)own;      // e / scale of 64 keys, then 2^-e
+        {
+          const uint32_t b = exps[64 + lane];
+          wave_sync();
+          ((float*)own)[lane] = ((float)b - 127.f) * inv_scale;
+          ((float*)own)[64 + lane] = __uint_as_float((254 - b) << 23);
+          wave_sync();
+        }
+        f32x4 x[NR][NU], inv[NU];
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+          const f32x4 ev = mine[4 * u + l4];
+          inv[u] = mine[16 + 4 * u + l4];
+          const int ke = exps[16 * u + l15];
+#pragma unroll
+          for (int k = 0; k < W::KS; ++k) {
+            i32x8 kf = {};
+#pragma unroll
+            for (int j = 0; j < 2 && 128 * k + 64 * j < DK; ++j) {
+              const int row = 16 * u + l15;
+              const i32x4 w = *(const i32x4*)(kt + row * DK + (((8 * k + 4 * j + l4) ^ key_swizzle<DK>(row)) << 4));
+#pragma unroll
+              for (int m = 0; m < 4; ++m) kf[4 * j + m] = w[m];
+            }
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                x[i][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qc[i][h][k], h == 0 && k == 0 ? ev : x[i][u], 0, 0, 0, ke, 0, qe[i][h]);
+          }
+        }
+        f16x4 pq[NR][NU];
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+          if (edge) {
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, 16 * u + 4 * l4 + r) ? x[i][u][r] : NEG;
+          }
+          softmax(i, x[i], inv, No(), 1.f);
+#pragma unroll
+          for (int u = 0; u < NU; ++u) pq[i][u] = (f16x4){(_Float16)x[i][u][0], (_Float16)x[i][u][1], (_Float16)x[i][u][2], (_Float16)x[i][u][3]};
+        }
+        const int base = code_column<DV>(l15, l4);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < NVB; ++c) {
+            const f16x8 vf = code_halves(read_code_column<DV>(vt, base, h, c));
+#pragma unroll
+            for (int i = 0; i < NR; ++i)
+              acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_shufflevector(pq[i][2 * h], pq[i][2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7), acc[i][c], 0, 0, 0);
+          }
+        if (bad) {
+          const uint8_t* vb = p.vc + at * DV;
+#pragma unroll
+          for (int i = 0; i < NR; ++i) {
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (!seen(i, 16 * u + 4 * l4 + r)) x[i][u][r] = -1.f;
+            add_nonfinite(i, x[i], [&](int j, int d) { return j >= lo && j < hi && (vb[j * DV + d] & 127) == 127 ? __builtin_nanf("") : 0.f; });
+          }
+        }
+      }
+    }
+  }
+
+  // ---- the drafted tokens: the last part ----
+  if (s.split == p.nsplit - 1) {
+    typedef Wide<DK, DV, NW, false> E;      // 32 keys of elements in the ring's memory
+    frag_t q[NR][DK / 32];
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+      for (int k = 0; k < DK / 32; ++k) q[i][k] = row_ok[i] ? *(const frag_t*)(qrow[i] + 32 * k + 8 * l4) : frag_t{};
+    for (int j0 = 0; j0 < s.drafted; j0 += 32) {
+      const int rows = min(s.drafted - j0, 32);
+      const int64_t row0 = s.f0 + j0;
+      uint8_t* kt = lds;
+      uint8_t* vt = lds + E::KBYTES;
+      __syncthreads();      // what was there has been read
+      for (int i = tid; i < 32 * DK / 8; i += 64 * NW) {
+        const int row = i / (DK / 8), c = i % (DK / 8);
+        *(frag_t*)(kt + W::KTile::slot(row, c)) = *(const frag_t*)(p.k + (row0 + min(row, rows - 1)) * p.ldk + (int64_t)s.g * DK + 8 * c);
+      }
+      for (int i = tid; i < 32 * DV / 8; i += 64 * NW) {
+        const int row = i / (DV / 8), c = i % (DV / 8);
+        *(frag_t*)(vt + W::VT::slot(row, c)) = *(const frag_t*)(p.v + (row0 + min(row, rows - 1)) * p.ldv + (int64_t)s.g * DV + 8 * c);
+      }
+      __syncthreads();
+      int e;
+      const bool bad = clean_elems(vt, 0, rows, e);
+      if (!live) continue;
+      uint32_t bits[NR];
+      int kpos[2][4];
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+        bits[i] = row_ok[i] && (j0 >> 6) < p.words ? (uint32_t)(p.mask[(int64_t)token[i] * p.words + (j0 >> 6)] >> (j0 & 63)) : 0u;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) kpos[u][r] = p.pos[min((int)row0 + 16 * u + 4 * l4 + r, s.f0 + s.drafted - 1)];
+      const elem_t* vb = p.v + row0 * p.ldv + (int64_t)s.g * DV;
+      elem_products(kt, vt, q, true, bad, e,
+                    [&](int i, int key) {      // (key is a constant plus 4 l4)
+                      const int u = (key - 4 * l4) >> 4, r = (key - 4 * l4) & 3;
+                      return (bool)((int)(key < rows) & (int)(bits[i] >> key & 1) & (int)(kpos[u][r] > low[i]));
+                    },
+                    [&](int j, int d) { return j < rows ? (float)vb[j * p.ldv + d] : 0.f; });
+    }
+  }
+
+  // ---- results ----
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const float l = column_sum(l_run[i]);
+    if (!row_ok[i]) continue;
+    const int r = r0 + 16 * i + l15, tk = r / s.gs, h = s.g * s.gs + r - tk * s.gs;
+    if (p.nsplit > 1) {
+      const int64_t at = ((int64_t)(s.f0 + tk) * p.H + h) * p.nsplit + s.split;
+#pragma unroll
+      for (int c = 0; c < NVB; ++c) *(f32x4*)(p.part + at * DV + 16 * c + 4 * l4) = acc[i][c];
+      if (l4 == 0) { p.ml[2 * at] = m_run[i]; p.ml[2 * at + 1] = l; }
+    } else {
+      const float f = l != 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+      for (int c = 0; c < NVB; ++c) *(quad_t*)(p.o + (int64_t)(s.f0 + tk) * p.ldo + (int64_t)h * DV + 16 * c + 4 * l4) = to_quad(acc[i][c] * f);
+    }
+  }
+}
+
+template <int DK, int DV, int NW, bool CODES>
+static int launch(TreeArgs& a, hipStream_t s) {
+  typedef Wide<DK, DV, NW, CODES> W;
+  const int rows = a.max_draft * (a.H / a.G);
+  a.blocks = (rows + W::ROWS - 1) / W::ROWS;
+  const int64_t groups = (int64_t)a.B * a.G * a.nsplit * a.blocks;
+  if (groups > 1 << 28) return LM_EINVAL;
+  constexpr int E = 32 * 2 * (DK + DV);      // a drafted tile
+  constexpr size_t bytes = W::LDS;
+  static_assert(W::NBUF * W::SLOT >= E, "a drafted tile fits the ring");
+  if (allow_lds(tree_wide_kernel<DK, DV, NW, CODES>, bytes) != LM_OK) return LM_EINVAL;
+  hipLaunchKernelGGL((tree_wide_kernel<DK, DV, NW, CODES>), dim3((unsigned)((groups + 7) / 8 * 8)), dim3(64 * NW), bytes, s, a);
+  return launch_status();
+}
+
+// Waves of a workgroup: as few as hold the rows, as many as share a tile
+static int waves(int rows, int dv) {
+  const int per = dv > 128 ? 16 : 32;
+  return rows <= 2 * per ? 2 : rows <= 4 * per ? 4 : 8;
+}
+
+bool tree_wide_takes(int rows, int dk, int dv) { return rows > (dv > 128 ? 16 : 32); }
+int tree_wide_rows(int rows, int dk, int dv) { return waves(rows, dv) * (dv > 128 ? 16 : 32); }
+
+int launch_tree_wide(TreeArgs& a, int dk, int dv, hipStream_t s) {
+  const int nw = waves(a.max_draft * (a.H / a.G), dv);
+  const bool codes = a.ke != nullptr;
+#define LM_CASE(K, V)                                                                               \
+  if (dk == K && dv == V) {                                                                         \
+    if (nw == 2) return codes ? launch<K, V, 2, true>(a, s) : launch<K, V, 2, false>(a, s);          \
+    if (nw == 4) return codes ? launch<K, V, 4, true>(a, s) : launch<K, V, 4, false>(a, s);          \
+    return codes ? launch<K, V, 8, true>(a, s) : launch<K, V, 8, false>(a, s);                       \
+  }
+  LM_CASE(64, 64) LM_CASE(64, 128) LM_CASE(64, 256) LM_CASE(128, 64) LM_CASE(128, 128) LM_CASE(128, 256)
+  LM_CASE(256, 64) LM_CASE(256, 128) LM_CASE(256, 256)
+#undef LM_CASE
+  return LM_EINVAL;
+}
+#else
+// f32, the format of verification, has the one kernel
+bool tree_wide_takes(int, int, int) { return false; }
+int tree_wide_rows(int, int, int) { return 1; }
+int launch_tree_wide(TreeArgs&, int, int, hipStream_t) { return LM_EINVAL; }
+#endif
+
+}  // namespace lm

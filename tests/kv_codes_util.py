@@ -53,12 +53,13 @@ def quantised(x, device):
 
 
 def attention(q, k, v, mask, first, pos, kpool, vpool, bt, length, scale, window, max_draft, groups):
-    """-> (output, sum p |v|, largest scale * sum |q| |k|, largest p * row's max |v|, seen keys), all of [tokens, heads, ..]; pools [pages, G, 64, size] f64;
+    """-> (output, sum p |v|, largest scale * sum |q| |k|, largest p * row's max |v|, seen keys, largest scale * max |q| * sum |k|), all of [tokens, heads, ..]; pools [pages, G, 64, size] f64;
     rows of no sequence are NaN"""
     n, H, dk = q.shape
     G, dv = kpool.shape[1], vpool.shape[3]
     out = torch.full((n, H, dv), math.nan, dtype=torch.float64, device=q.device)
-    size, sums, peak, count = out.clone(), out[..., :1].clone(), out[..., :1].clone(), out[..., :1].clone()
+    size = out.clone()
+    sums, peak, count, coarse = (out[..., :1].clone() for _ in range(4))
     for b, ln in enumerate(length.tolist()):
         f0 = int(first[b])
         T = min(int(first[b + 1]) - f0, max_draft)
@@ -88,18 +89,23 @@ def attention(q, k, v, mask, first, pos, kpool, vpool, bt, length, scale, window
             val = torch.where(seen[..., None], vv[g][None], 0.0)
             out[f0:f0 + T, h] = (w[..., None] * val).sum(1)
             size[f0:f0 + T, h] = (w[..., None] * val.abs()).sum(1)
-            sums[f0:f0 + T, h, 0] = (torch.where(seen, (row.abs() @ kk[g].abs().nan_to_num(nan=0.0, posinf=0.0).T), 0.0)).amax(-1) * scale
+            mag = kk[g].abs().nan_to_num(nan=0.0, posinf=0.0)
+            sums[f0:f0 + T, h, 0] = torch.where(seen, row.abs() @ mag.T, 0.0).amax(-1) * scale
+            coarse[f0:f0 + T, h, 0] = torch.where(seen, row.abs().amax(-1, keepdim=True) * mag.sum(-1), 0.0).amax(-1) * scale
             peak[f0:f0 + T, h, 0] = (w * val.abs().amax(-1)).amax(-1)
             count[f0:f0 + T, h, 0] = seen.sum(-1).double()
-    return out, size, sums, peak, count
+    return out, size, sums, peak, count, coarse
 
 
-def attention_bound(dtype, codes, dk, ref, size, sums, peak, count):
+def attention_bound(dtype, codes, dk, ref, size, sums, peak, count, coarse):
     """How far lm_tree_attn may be from 64 bits: the result's rounding; then relative to sum p |v|: scores are sums of dk products in f32 (twice that
     for the order, and the conversion to a power of two), whose error enters every p and the total; a weight is 11 bits where values are codes (half a step
     2^-12, twice for the total's that is not rounded) and 16 of two bf16, or f32; exponentials and f32 sums of all keys.  Weights below 2^-39 of the
-    largest (times its values' power of two, at most 2^-7 of the row's largest value) are lost."""
+    largest (times its values' power of two, at most 2^-7 of the row's largest value) are lost.  Many rows over codes: a query element is two codes,
+    q = 2^e (hi + lo / 16), max |q| > 224 * 2^e; hi is off by at most half a step, 2^-4 of it or (below 2^-6) 2^-10, lo is 16 times that, at most 256, and off by 2^-10 where it is below
+    2^-6 and not at all where its 4 bits hold the rest (bf16 has 8): the element by 2^-14 * 2^e < 2^-21 max |q|; that times |k|, in every p and the total."""
     weight = (2.0 ** -12 if codes else 2.0 ** -16) if dtype == torch.bfloat16 else 2.0 ** -23
     rel = 2 * (dk + 4) * 2.0 ** -24 * (sums + 1.0) + weight + (count + 8) * 2.0 ** -24 + 2.0 ** -21
+    rel = rel + (2 * 2.0 ** -21 * coarse if codes and dtype == torch.bfloat16 else 0.0)
     lost = count * 2.0 ** -39 * peak * 448 / 224 if codes and dtype == torch.bfloat16 else 0.0
     return 1.01 * UNIT[dtype] * ref.abs() + rel * size + lost + 1e-30
