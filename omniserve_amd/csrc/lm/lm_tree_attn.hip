@@ -29,8 +29,7 @@ struct Tree {
   static constexpr int CH = DK / 64, PF = 16 / FR, NKF = CH * PF, NVB = DV / 16;
   static constexpr int KT = CODES ? 64 : 32, NU = KT / 16;        // keys of a context tile
   static constexpr int STAGE = 64 * DV;                           // bytes of a wave's V tile: 64 rows of codes, 32 of bf16
-  static constexpr int RED = 4 * 16 * (DV + 4) * 4, PBUF = 4 * 4096;
-  static constexpr int LDS = (SPLIT && 4 * STAGE > RED ? 4 * STAGE : RED) > PBUF ? (SPLIT && 4 * STAGE > RED ? 4 * STAGE : RED) : PBUF;
+  static constexpr int RED = 4 * 16 * (DV + 4) * 4, LDS = SPLIT && 4 * STAGE > RED ? 4 * STAGE : RED;
   typedef Tile<SPLIT ? DV * 2 : 256> VT;
 
   const TreeArgs& p;
@@ -77,29 +76,23 @@ struct Tree {
     }
   }
 
-  // What non-finite values of a tile in which not every row sees every key add: they were left out of the products, where a weight of
-  // zero would have made them NaN in rows that do not see them.  w: this lane's weights, -1 where unseen.
-  template <int U, typename Value>
-  __device__ __forceinline__ void add_nonfinite(f32x4 (&a)[NVB], const f32x4 (&w)[U], Value value) {
-    float* buf = (float*)stage;
-    wave_sync();
+  // What non-finite values among keys lo .. hi - 1 of a tile add to the rows that see them.  (They were left out of the products, where a weight of
+  // zero would have made them NaN in every row; a weight's size does not matter to them.)
+  template <typename Seen, typename Value>
+  __device__ __forceinline__ void add_nonfinite(int lo, int hi, Seen seen, Value value) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) buf[(16 * u + 4 * l4 + r) * 16 + l15] = w[u][r];
-    wave_sync();
+    for (int i = 0; i < NR; ++i)
 #pragma unroll 1
-    for (int j = 0; j < 16 * U; ++j) {
-      const float f = buf[16 * j + l15];
+      for (int j = max(lo, 0); j < hi; ++j) {
+        const bool see = seen(i, j);
 #pragma unroll
-      for (int c = 0; c < NVB; ++c)
+        for (int c = 0; c < NVB; ++c)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float y = value(j, 16 * c + 4 * l4 + r);
-          if (f >= 0.f && !(fabsf(y) < __builtin_inff())) a[c][r] += f * y;
-        }
-    }
-    wave_sync();
+          for (int r = 0; r < 4; ++r) {
+            const float y = value(j, 16 * c + 4 * l4 + r);
+            acc[i][c][r] += (int)see & (int)!(fabsf(y) < __builtin_inff()) ? y : 0.f;
+          }
+      }
   }
 
   // ---- context tiles of codes ----
@@ -250,17 +243,7 @@ struct Tree {
     }
     if (bad) {
       const uint8_t* vb = p.vc + here * DV;
-#pragma unroll
-      for (int i = 0; i < NR; ++i) {
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int key = 16 * u + 4 * l4 + r;
-            if (!((int)(key >= lo) & (int)(key < hi) & (int)(kb + key > low[i]))) x[i][u][r] = -1.f;
-          }
-        add_nonfinite<NU>(acc[i], x[i], [&](int j, int d) { return j >= lo && j < hi && (vb[j * DV + d] & 127) == 127 ? __builtin_nanf("") : 0.f; });
-      }
+      add_nonfinite(lo, min(hi, KT), [&](int i, int j) { return kb + j > low[i]; }, [&](int j, int d) { return (vb[j * DV + d] & 127) == 127 ? __builtin_nanf("") : 0.f; });
     }
   }
 
@@ -387,17 +370,7 @@ struct Tree {
         for (int m = 0; m < NOPND; ++m) acc[i][cb] = mma_quads(v[0], v[1], pq[i][0][m], pq[i][1][m], acc[i][cb]);
     }
     if constexpr (!SPLIT) bad = __any(bad);
-    if (bad) {
-#pragma unroll
-      for (int i = 0; i < NR; ++i) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (!seen(i, 16 * u + 4 * l4 + r)) x[i][u][r] = -1.f;
-        add_nonfinite<2>(acc[i], x[i], [&](int j, int d) { return j >= lo && j < hi ? (float)vp[j * ldv + d] : 0.f; });
-      }
-    }
+    if (bad) add_nonfinite(lo, min(hi, 32), seen, [&](int j, int d) { return (float)vp[j * ldv + d]; });
   }
 };
 
@@ -414,7 +387,7 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
   T t(p);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   t.lane = tid & 63; t.l15 = tid & 15; t.l4 = (tid & 63) >> 4;
-  t.stage = lds + wave * (SPLIT ? T::STAGE : 4096);
+  t.stage = lds + wave * (SPLIT ? T::STAGE : 0);
   int low_min = INT32_MAX, low_max = INT32_MIN, token[NR];
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
@@ -494,19 +467,13 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
       const int64_t row = f0 + j0;
       t.load_elems(c, p.k + row * p.ldk + (int64_t)g * DK, p.ldk, p.v + row * p.ldv + (int64_t)g * DV, p.ldv, min(drafted - j0, 32));
       uint32_t bits[NR];
-      int kpos[2][4];
 #pragma unroll
       for (int i = 0; i < NR; ++i)
         bits[i] = t.row_ok[i] && (j0 >> 6) < p.words ? (uint32_t)(p.mask[(int64_t)token[i] * p.words + (j0 >> 6)] >> (j0 & 63)) : 0u;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) kpos[u][r] = p.pos[min((int)row + 16 * u + 4 * t.l4 + r, f0 + drafted - 1)];
       const int hi = min(drafted - j0, 32);
       t.elem_tile(c, 0, hi, true,
-                  [&](int i, int key) {      // (key is a constant plus 4 l4)
-                    const int u = (key - 4 * t.l4) >> 4, r = (key - 4 * t.l4) & 3;
-                    return (bool)((int)(key < hi) & (int)(bits[i] >> key & 1) & (int)(kpos[u][r] > t.low[i]));
+                  [&](int i, int key) {
+                    return (bool)((int)(key < hi) & (int)(bits[i] >> key & 1) & (int)(p.pos[min((int)row + key, f0 + drafted - 1)] > t.low[i]));
                   },
                   []() {});
     }
@@ -597,7 +564,7 @@ static int launch_tree(TreeArgs& a, hipStream_t s) {
   if (groups > 1 << 28) return LM_EINVAL;
   const dim3 grid((unsigned)((groups + 7) / 8 * 8));
   if (nr == 1) hipLaunchKernelGGL((tree_attn_kernel<DK, DV, 1, CODES>), grid, dim3(256), 0, s, a);
-  if constexpr (SPLIT && DV <= 128)
+  if constexpr (SPLIT && DK <= 128 && DV <= 128)
     if (nr == 2) hipLaunchKernelGGL((tree_attn_kernel<DK, DV, 2, CODES>), grid, dim3(256), 0, s, a);
   return launch_status();
 }

@@ -24,16 +24,19 @@ __device__ __forceinline__ int key_swizzle(int row) {
   else return Tile<ROWB>::swizzle(row);
 }
 
+// Blocks of 16 rows of a wave: what 256 registers hold
+constexpr int row_blocks(int dk, int dv) { return dk > 128 || dv > 128 ? 1 : 2; }
+
 template <int DK, int DV, int NW, bool CODES>
 struct Wide {
-  static constexpr int NR = DV > 128 ? 1 : 2, ROWS = NW * 16 * NR, NVB = DV / 16;
+  static constexpr int NR = row_blocks(DK, DV), ROWS = NW * 16 * NR, NVB = DV / 16;
   static constexpr int KT = CODES ? 64 : 32, NU = KT / 16;
   static constexpr int KB = CODES ? DK : 2 * DK, VB = CODES ? DV : 2 * DV;      // bytes of a row
   static constexpr int KBYTES = KT * KB, VBYTES = KT * VB, EXPS = CODES ? 128 : 0;
   static constexpr int SLOT = KBYTES + VBYTES + EXPS;                            // of the ring
   static constexpr int NBUF = NW == 2 ? 2 : 3;
-  static constexpr int KP = KBYTES / 1024, VP = VBYTES / 1024, EACH = (KP + VP + NW - 1) / NW, PIECES = EACH + (CODES ? 1 : 0);      // of a wave
-  static constexpr int OWN = 4096;                                               // a wave's: exponents; weights of a tile with non-finite values
+  static constexpr int KP = KBYTES / 1024, VP = VBYTES / 1024, EACH = (KP + VP + NW - 1) / NW, PIECES = EACH + (CODES ? 2 : 0);      // of a wave
+  static constexpr int OWN = CODES ? 512 : 0;                                     // a wave's: keys' exponents
   static constexpr int LDS = NBUF * SLOT + NW * OWN + 64;
   static constexpr int KS = CODES ? (DK + 127) / 128 : DK / 32;                  // steps of a key's product
   static constexpr float SHIFT = CODES ? 14.f : 0.f;
@@ -55,19 +58,19 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   const bool live = r0 < s.R;                                         // (a wave without rows fetches its pieces and waits with the others)
 
   // ---- rows ----
-  int low[NR], token[NR], low_min = INT32_MAX, low_max = INT32_MIN;
-  bool row_ok[NR];
-  const elem_t* qrow[NR];
+  auto token_of = [&](int i) { return s.f0 + min(r0 + 16 * i + l15, s.R - 1) / s.gs; };
+  auto query_of = [&](int i) {
+    const int tk = token_of(i);
+    return p.q + (int64_t)tk * p.ldq + (int64_t)(s.g * s.gs + min(r0 + 16 * i + l15, s.R - 1) - (tk - s.f0) * s.gs) * DK;
+  };
+  auto row_ok = [&](int i) { return r0 + 16 * i + l15 < s.R; };
+  int low[NR], low_min = INT32_MAX, low_max = INT32_MIN;
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
-    const int r = r0 + 16 * i + l15, rc = min(r, s.R - 1), tk = rc / s.gs;
-    token[i] = s.f0 + tk;
-    row_ok[i] = r < s.R;
-    const int lo = p.pos[token[i]] - p.window;
+    const int lo = p.pos[token_of(i)] - p.window;
     low_min = min(low_min, lo);
     low_max = max(low_max, lo);
-    low[i] = r < s.R ? lo : INT32_MAX;
-    qrow[i] = p.q + (int64_t)token[i] * p.ldq + (int64_t)(s.g * s.gs + rc - tk * s.gs) * DK;
+    low[i] = row_ok(i) ? lo : INT32_MAX;
   }
   if (tid == 0) { shared[0] = INT32_MAX; shared[1] = INT32_MIN; }
   __syncthreads();
@@ -87,7 +90,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   // Offsets of this lane's pieces: place in the slot -> byte of the tile in memory
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
   auto piece_of = [&](int j) { return min(j * NW + wave, W::KP + W::VP - 1); };      // (the last piece twice where they do not divide: equal bytes)
-  int from[W::EACH];
+  uint32_t from[W::EACH];
 #pragma unroll
   for (int j = 0; j < W::EACH; ++j) {
     const int pc = piece_of(j), key = pc < W::KP, at = (key ? pc : pc - W::KP) * 1024 + lane * 16, rowb = key ? W::KB : W::VB, row = at / rowb;
@@ -100,10 +103,13 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
     for (int j = 0; j < W::EACH; ++j) {
       const int pc = piece_of(j);
-      dma16_uncounted((pc < W::KP ? p.kc + at * W::KB : p.vc + at * W::VB) + from[j], to + pc * 1024);
+      dma16_uncounted(pc < W::KP ? p.kc + at * W::KB : p.vc + at * W::VB, from[j], to + pc * 1024);
     }
     if constexpr (CODES)      // (every wave, so that all have as many pieces in flight: the same bytes to the same place)
-      if (lane < 8) dma16_uncounted((lane < 4 ? p.ke : p.ve) + at + 16 * (lane & 3), to + W::KBYTES + W::VBYTES);
+      if (lane < 4) {
+        dma16_uncounted(p.ke + at, 16 * lane, to + W::KBYTES + W::VBYTES);
+        dma16_uncounted(p.ve + at, 16 * lane, to + W::KBYTES + W::VBYTES + 64);
+      }
   };
   constexpr int PER_PAGE = PAGE / KT;
   // (scalar loads: a vector load's wait would take in the DMA behind it)
@@ -122,6 +128,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   frag_t qf[NR][CODES ? 1 : W::KS];
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
+    const elem_t* qrow = query_of(i);
     if constexpr (CODES) {
       float y[W::KS][32], top = 0.f;
 #pragma unroll
@@ -130,7 +137,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const frag_t f = row_ok[i] && 128 * k + 64 * j < DK ? *(const frag_t*)(qrow[i] + 128 * k + 64 * j + 16 * l4 + 8 * h) : frag_t{};
+            const frag_t f = row_ok(i) && 128 * k + 64 * j < DK ? *(const frag_t*)(qrow + 128 * k + 64 * j + 16 * l4 + 8 * h) : frag_t{};
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               y[k][16 * j + 8 * h + e] = (float)f[e];
@@ -156,7 +163,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
         }
     } else {
 #pragma unroll
-      for (int k = 0; k < W::KS; ++k) qf[i][k] = row_ok[i] ? *(const frag_t*)(qrow[i] + 32 * k + 8 * l4) : frag_t{};
+      for (int k = 0; k < W::KS; ++k) qf[i][k] = row_ok(i) ? *(const frag_t*)(qrow + 32 * k + 8 * l4) : frag_t{};
     }
   }
 
@@ -203,31 +210,23 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   };
-  // What a tile's non-finite values add (lm_tree_attn.hip): x: weights, -1 where unseen
-  auto add_nonfinite = [&](int i, const auto& x, auto value) {
-    constexpr int U = sizeof(x) / sizeof(f32x4);
-    float* buf = (float*)own;
-    wave_sync();
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) buf[(16 * u + 4 * l4 + r) * 16 + l15] = x[u][r];
-    wave_sync();
+  // What non-finite values among keys lo .. hi - 1 of a tile add to the rows that see them.  (They were left out of the products, where a weight of
+  // zero would have made them NaN in every row; a weight's size does not matter to them.)
+  auto add_nonfinite = [&](int i, int lo, int hi, auto seen, auto value) {
 #pragma unroll 1
-    for (int j = 0; j < 16 * U; ++j) {
-      const float f = buf[16 * j + l15];
+    for (int j = max(lo, 0); j < hi; ++j) {
+      const bool see = seen(i, j);
 #pragma unroll
       for (int c = 0; c < NVB; ++c)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float y = value(j, 16 * c + 4 * l4 + r);
-          if (f >= 0.f && !(fabsf(y) < __builtin_inff())) acc[i][c][r] += f * y;
+          acc[i][c][r] += (int)see & (int)!(fabsf(y) < __builtin_inff()) ? y : 0.f;
         }
     }
-    wave_sync();
   };
   // A tile of 32 keys and values in elements at `tile`: products, weights, products
-  auto elem_products = [&](const uint8_t* kt, const uint8_t* vt, const frag_t (&q)[NR][DK / 32], bool edge, bool bad, int e, auto seen, auto value) {
+  auto elem_products = [&](const uint8_t* kt, const uint8_t* vt, const frag_t (&q)[NR][DK / 32], bool edge, bool bad, int e, int lo, int hi, auto seen, auto value) {
     f32x4 x[NR][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -260,14 +259,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
     }
     if (bad) {
 #pragma unroll
-      for (int i = 0; i < NR; ++i) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (!seen(i, 16 * u + 4 * l4 + r)) x[i][u][r] = -1.f;
-        add_nonfinite(i, x[i], value);
-      }
+      for (int i = 0; i < NR; ++i) add_nonfinite(i, lo, hi, seen, value);
     }
   };
   // Values of a tile that not every row sees: rows outside lo .. hi - 1 and non-finite ones become zero; elements are divided by 2^e (codes' kernel).
@@ -337,7 +329,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       }
       if (live) {
         const elem_t* vb = (const elem_t*)p.vc + at * DV;
-        elem_products(kt, vt, qf, edge, bad, 0, seen, [&](int j, int d) { return j >= lo && j < hi ? (float)vb[j * DV + d] : 0.f; });
+        elem_products(kt, vt, qf, edge, bad, 0, lo, min(hi, KT), seen, [&](int j, int d) { return (float)vb[j * DV + d]; });
       }
     } else {
       uint8_t* exps = vt + W::VBYTES;
@@ -389,6 +381,17 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
                 x[i][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qc[i][h][k], h == 0 && k == 0 ? ev : x[i][u], 0, 0, 0, ke, 0, qe[i][h]);
           }
         }
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+          for (int u = 0; u < NU; ++u) asm volatile("" : "+v"(x[i][u]));      // (not later: the keys' registers are free here)
+        // A column's read is requested eight products ahead: its latency is as long as six of them
+        const int base = code_column<DV>(l15, l4);
+        constexpr int AHEAD = NVB < 8 ? NVB : 8;
+        u32x2 w[AHEAD];
+#pragma unroll
+        for (int c = 0; c < AHEAD; ++c) w[c] = read_code_column<DV>(vt, base, 0, c);
+        __builtin_amdgcn_sched_barrier(0);
         f16x4 pq[NR][NU];
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
@@ -402,12 +405,12 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
           for (int u = 0; u < NU; ++u) pq[i][u] = (f16x4){(_Float16)x[i][u][0], (_Float16)x[i][u][1], (_Float16)x[i][u][2], (_Float16)x[i][u][3]};
         }
-        const int base = code_column<DV>(l15, l4);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int c = 0; c < NVB; ++c) {
-            const f16x8 vf = code_halves(read_code_column<DV>(vt, base, h, c));
+            const f16x8 vf = code_halves(w[c % AHEAD]);
+            if (h * NVB + c + AHEAD < 2 * NVB) w[c % AHEAD] = read_code_column<DV>(vt, base, c + AHEAD < NVB ? h : 1, (c + AHEAD) % NVB);
 #pragma unroll
             for (int i = 0; i < NR; ++i)
               acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_shufflevector(pq[i][2 * h], pq[i][2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7), acc[i][c], 0, 0, 0);
@@ -415,14 +418,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
         if (bad) {
           const uint8_t* vb = p.vc + at * DV;
 #pragma unroll
-          for (int i = 0; i < NR; ++i) {
-#pragma unroll
-            for (int u = 0; u < NU; ++u)
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (!seen(i, 16 * u + 4 * l4 + r)) x[i][u][r] = -1.f;
-            add_nonfinite(i, x[i], [&](int j, int d) { return j >= lo && j < hi && (vb[j * DV + d] & 127) == 127 ? __builtin_nanf("") : 0.f; });
-          }
+          for (int i = 0; i < NR; ++i) add_nonfinite(i, lo, min(hi, KT), seen, [&](int j, int d) { return (vb[j * DV + d] & 127) == 127 ? __builtin_nanf("") : 0.f; });
         }
       }
     }
@@ -433,9 +429,11 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
     typedef Wide<DK, DV, NW, false> E;      // 32 keys of elements in the ring's memory
     frag_t q[NR][DK / 32];
 #pragma unroll
-    for (int i = 0; i < NR; ++i)
+    for (int i = 0; i < NR; ++i) {
+      const elem_t* qrow = query_of(i);
 #pragma unroll
-      for (int k = 0; k < DK / 32; ++k) q[i][k] = row_ok[i] ? *(const frag_t*)(qrow[i] + 32 * k + 8 * l4) : frag_t{};
+      for (int k = 0; k < DK / 32; ++k) q[i][k] = row_ok(i) ? *(const frag_t*)(qrow + 32 * k + 8 * l4) : frag_t{};
+    }
     for (int j0 = 0; j0 < s.drafted; j0 += 32) {
       const int rows = min(s.drafted - j0, 32);
       const int64_t row0 = s.f0 + j0;
@@ -455,21 +453,15 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       const bool bad = clean_elems(vt, 0, rows, e);
       if (!live) continue;
       uint32_t bits[NR];
-      int kpos[2][4];
 #pragma unroll
       for (int i = 0; i < NR; ++i)
-        bits[i] = row_ok[i] && (j0 >> 6) < p.words ? (uint32_t)(p.mask[(int64_t)token[i] * p.words + (j0 >> 6)] >> (j0 & 63)) : 0u;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) kpos[u][r] = p.pos[min((int)row0 + 16 * u + 4 * l4 + r, s.f0 + s.drafted - 1)];
+        bits[i] = row_ok(i) && (j0 >> 6) < p.words ? (uint32_t)(p.mask[(int64_t)token_of(i) * p.words + (j0 >> 6)] >> (j0 & 63)) : 0u;
       const elem_t* vb = p.v + row0 * p.ldv + (int64_t)s.g * DV;
-      elem_products(kt, vt, q, true, bad, e,
-                    [&](int i, int key) {      // (key is a constant plus 4 l4)
-                      const int u = (key - 4 * l4) >> 4, r = (key - 4 * l4) & 3;
-                      return (bool)((int)(key < rows) & (int)(bits[i] >> key & 1) & (int)(kpos[u][r] > low[i]));
+      elem_products(kt, vt, q, true, bad, e, 0, rows,
+                    [&](int i, int key) {
+                      return (bool)((int)(key < rows) & (int)(bits[i] >> key & 1) & (int)(p.pos[min((int)row0 + key, s.f0 + s.drafted - 1)] > low[i]));
                     },
-                    [&](int j, int d) { return j < rows ? (float)vb[j * p.ldv + d] : 0.f; });
+                    [&](int j, int d) { return (float)vb[j * p.ldv + d]; });
     }
   }
 
@@ -477,7 +469,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     const float l = column_sum(l_run[i]);
-    if (!row_ok[i]) continue;
+    if (!row_ok(i)) continue;
     const int r = r0 + 16 * i + l15, tk = r / s.gs, h = s.g * s.gs + r - tk * s.gs;
     if (p.nsplit > 1) {
       const int64_t at = ((int64_t)(s.f0 + tk) * p.H + h) * p.nsplit + s.split;
@@ -508,16 +500,16 @@ static int launch(TreeArgs& a, hipStream_t s) {
 }
 
 // Waves of a workgroup: as few as hold the rows, as many as share a tile
-static int waves(int rows, int dv) {
-  const int per = dv > 128 ? 16 : 32;
+static int waves(int rows, int dk, int dv) {
+  const int per = 16 * row_blocks(dk, dv);
   return rows <= 2 * per ? 2 : rows <= 4 * per ? 4 : 8;
 }
 
-bool tree_wide_takes(int rows, int dk, int dv) { return rows > (dv > 128 ? 16 : 32); }
-int tree_wide_rows(int rows, int dk, int dv) { return waves(rows, dv) * (dv > 128 ? 16 : 32); }
+bool tree_wide_takes(int rows, int dk, int dv) { return rows > 16 * row_blocks(dk, dv); }
+int tree_wide_rows(int rows, int dk, int dv) { return waves(rows, dk, dv) * 16 * row_blocks(dk, dv); }
 
 int launch_tree_wide(TreeArgs& a, int dk, int dv, hipStream_t s) {
-  const int nw = waves(a.max_draft * (a.H / a.G), dv);
+  const int nw = waves(a.max_draft * (a.H / a.G), dk, dv);
   const bool codes = a.ke != nullptr;
 #define LM_CASE(K, V)                                                                               \
   if (dk == K && dv == V) {                                                                         \
