@@ -95,13 +95,14 @@ int lm_kv_load(void* k, int64_t ldk, void* v, int64_t ldv, const uint8_t* kc, co
 /* Attention of drafted tokens: sequence b has tokens first[b] .. first[b + 1] - 1 of q [H][dk], k [G][dk], v [G][dv] (positions pos, turned
  * already; at most max_draft, further ones are left out) and length[b] keys in the pages bt[b].  A token sees the context, and drafted token j of its sequence
  * where bit j % 64 of mask[token][j / 64] is set, both only from position pos - window + 1 on.  It sees nothing: zeros.  Pools as above, or
- * (ke, ve null) of elem; pages outside 0 .. pages - 1 are not seen.  part: f32 [n * H * nsplit * (dv + 2)] for nsplit > 1;
- * lm_tree_attn_splits: how many parts suit (max_context: bound of the lengths, a hint). */
-int lm_tree_attn_splits(int B, int max_draft, int max_context, int H, int G, int dk, int dv);
+ * (ke, ve null) of elem; pages outside 0 .. pages - 1 are not seen.  part: lm_tree_attn_scratch() f32 for these
+ * sizes, by which the keys of few or unequal sequences are dealt out (null: a workgroup has all keys of its rows); max_context: bound of the
+ * lengths, a hint.  window INT32_MAX: none. */
+int64_t lm_tree_attn_scratch(int B, int max_draft, int max_context, int H, int G, int dk, int dv, int codes);
 int lm_tree_attn(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const void* kc, const void* vc,
                  const uint8_t* ke, const uint8_t* ve, int64_t pages, const int* bt, int bt_stride, int bt_width, const int* length,
-                 const int* first, const int* pos, const int64_t* mask, int words, void* o, int64_t ldo, float* part, int nsplit, float scale,
-                 int window, int B, int n, int max_draft, int H, int G, int dk, int dv, void* stream);
+                 const int* first, const int* pos, const int64_t* mask, int words, void* o, int64_t ldo, float* part, float scale, int window,
+                 int B, int n, int max_draft, int max_context, int H, int G, int dk, int dv, void* stream);
 
 /* Decayed linear attention; rows q [H][dk] k [H][dk] v [H][dv], `act` applied to all three.  seg [.][8]: first token, tokens,
  * slot, starts from zero, index in its entry, segments of the entry, 0, 0; all but an entry's last have seg_len tokens.

@@ -49,9 +49,9 @@ PROTOTYPES = {
     "lm_rope": (_i, [_vp, _i64, _vp, _i64, _vp, _i, _vp, _i, _f, _i, _i, _i, _vp]),
     "lm_kv_store": (_i, [_vp, _i64, _i, _vp, _vp, _i, _vp, _i, _f, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
     "lm_kv_load": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i, _i, _i, _i, _vp]),
-    "lm_tree_attn_splits": (_i, [_i] * 7),
-    "lm_tree_attn": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _i64, _vp, _i, _f,
-                          _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "lm_tree_attn_scratch": (_i64, [_i] * 8),
+    "lm_tree_attn": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _i64, _vp, _f,
+                          _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "lm_linear_prefill": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _i, _i, _i, _vp]),
     "lm_linear_decode": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "lm_latent_append": (_i, [_vp, _i64, _i64, _vp, _f, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
@@ -200,7 +200,7 @@ class LmOps:
     def _x(self):
         if self._bound is None:
             at = lambda name: _c.cast(getattr(self._h, name), _vp).value      # noqa: E731
-            self._bound = _binding().Ops(self.dtype == torch.bfloat16, *map(at, ("lm_rope", "lm_kv_store", "lm_kv_load", "lm_tree_attn_splits", "lm_tree_attn")))
+            self._bound = _binding().Ops(self.dtype == torch.bfloat16, *map(at, ("lm_rope", "lm_kv_store", "lm_kv_load", "lm_tree_attn_scratch", "lm_tree_attn")))
         return self._bound
 
     def rope(self, x, freq, pos, heads, dk, *, pairing="neighbours", factor=1.0, out=None):

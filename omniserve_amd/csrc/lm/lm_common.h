@@ -206,6 +206,8 @@ __device__ __forceinline__ void dma16_uncounted(const void* src, uint32_t lds_ds
 __device__ __forceinline__ void dma16_uncounted(const void* base, uint32_t off, uint32_t lds_dst) {
   uint32_t keep;
   lds_dst = __builtin_amdgcn_readfirstlane(lds_dst);
+  const uint64_t at = (uint64_t)base;
+  base = (const void*)((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at));
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
                : "=&s"(keep)
                : "v"(off), "s"(base), "s"(lds_dst)

@@ -1,6 +1,7 @@
 // What the two kernels of drafted tokens' attention share (lm_tree_attn.hip: few rows, lm_tree_wide.hip: many).
 #pragma once
 #include "lm_attn.h"
+#include <initializer_list>
 #include "lm_kv_codes.h"
 
 namespace lm {
@@ -19,10 +20,28 @@ struct TreeArgs {
   const int* length; const int* first; const int* pos;
   const unsigned long long* mask; int words;
   elem_t* o; int64_t ldo;
-  float* ml; float* part;                            // nsplit > 1: [n * H][nsplit][2] and [n * H][nsplit][dv]
+  float* ml; float* part;                            // of cut pieces: [workgroups][rows][2] and [workgroups][rows][dv]; null: nothing is cut
   float scale;                                       // includes log2(e)
-  int window, n, H, G, B, nsplit, max_draft, blocks;
+  int window;                                        // NO_WINDOW: none
+  int n, H, G, B, max_draft, blocks, workgroups;     // blocks: of rows, the most a sequence has
 };
+constexpr int NO_WINDOW = INT32_MAX;
+
+// The newest position that a token does not see any more
+__device__ __forceinline__ int bound_of(const TreeArgs& p, int pos) { return p.window == NO_WINDOW ? INT32_MIN : max(pos, INT32_MIN + p.window) - p.window; }
+
+// Largest of the four lanes that share l15, by lane swaps (column_max goes through LDS: two latencies in every tile's chain)
+__device__ __forceinline__ float rows_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+// x in a place that few tiles come to: nothing formed from it moves in front of the branch
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 
 // The 16-byte slot of a row of dv codes in LDS, so that the eight rows of both 16-lane groups of a transposed read lie in different banks.
 template <int DV>
@@ -63,28 +82,138 @@ __device__ __forceinline__ uint32_t drop_nan_codes(uint32_t w, bool& bad) {
   return w & ~(nan - (nan >> 7) | nan);
 }
 
-// Which sequence's tokens, rows and keys a workgroup has
-struct Share {
-  int rb, split, g, b, f0, drafted, gs, R, length;
-  const int* bt;
+// ---- how the work is dealt out ----
+// A segment is the keys of one (sequence, kv head, block of rows): its context tiles that any row sees and, behind them, tiles of 32 drafted tokens.
+// Where segments are few or of different lengths they are cut into equal pieces of at most run_length() tiles, a workgroup each.  The length follows from
+// the tiles of all of them, so that there are as many pieces as suit the chip whatever the sequences' lengths are (a fixed number of parts a sequence
+// leaves the short ones' places idle).  A segment of one piece is written by it, others are joined by tree_merge_kernel.  The division depends on the
+// lengths alone.
+constexpr int RUN = 4;      // tiles of a piece at least, where it is not all of its segment (for each of the narrow kernel's waves one)
+
+struct Segments {            // of one sequence
+  int f0, drafted, length, t0, nt, nd, blocks;
+  __device__ __forceinline__ int tiles() const { return nt + nd; }
 };
-__device__ __forceinline__ bool share_of(const TreeArgs& p, Share& s, int rows) {
-  const int id = xcd_contiguous(blockIdx.x, p.B * p.G * p.nsplit * p.blocks);
-  if (id < 0) return false;
-  // row blocks of the same keys are neighbours: one XCD's L2 serves them
-  s.rb = id % p.blocks; s.split = id / p.blocks % p.nsplit; s.g = id / p.blocks / p.nsplit % p.G; s.b = id / p.blocks / p.nsplit / p.G;
-  s.f0 = min(max(p.first[s.b], 0), p.n);
-  s.drafted = min(max(p.first[s.b + 1] - s.f0, 0), min(p.max_draft, p.n - s.f0));
-  s.gs = p.H / p.G;
-  s.R = s.drafted * s.gs;
-  s.length = min(max(p.length[s.b], 0), p.bt_width * PAGE);
-  s.bt = p.bt + (int64_t)s.b * p.bt_stride;
-  return s.rb * rows < s.R;
+template <int KT, int ROWS>
+__device__ __forceinline__ Segments segments_of(const TreeArgs& p, int b) {
+  Segments q;
+  q.f0 = min(max(p.first[b], 0), p.n);
+  q.drafted = min(max(p.first[b + 1] - q.f0, 0), min(p.max_draft, p.n - q.f0));
+  q.length = min(max(p.length[b], 0), p.bt_width * PAGE);
+  q.blocks = (q.drafted * (p.H / p.G) + ROWS - 1) / ROWS;
+  int low = INT32_MIN;
+  if (p.window != NO_WINDOW && q.drafted > 0) {
+    low = INT32_MAX;
+    for (int i = 0; i < q.drafted; ++i) low = min(low, bound_of(p, p.pos[q.f0 + i]));
+  }
+  q.t0 = min(max(low, -1) + 1, q.length) / KT;
+  q.nt = (q.length + KT - 1) / KT - q.t0;
+  q.nd = (q.drafted + 31) / 32;
+  return q;
 }
 
-// Many rows (lm_tree_wide.hip): returns false where the kernel does not exist
+__device__ __forceinline__ int pieces_of(const Segments& q, int run) { return (q.tiles() + run - 1) / run; }      // of one segment
+
+// All sequences, 64 at a time, a lane each; the first 64 are looked up once
+template <int KT, int ROWS>
+struct Batch {
+  const TreeArgs& p;
+  Segments mine;
+  int lane;
+  __device__ __forceinline__ Batch(const TreeArgs& a) : p(a), lane(threadIdx.x & 63) { mine = look(lane); }
+  __device__ __forceinline__ Segments look(int b) const {
+    Segments q{};
+    if (b < p.B) q = segments_of<KT, ROWS>(p, b);
+    return q;
+  }
+  __device__ __forceinline__ Segments at(int b0) const { return b0 == 0 ? mine : look(b0 + lane); }
+  // f(segments) times heads and row blocks, summed over the sequences in front of `upto`
+  template <typename F>
+  __device__ __forceinline__ uint32_t sum(int upto, F f) const {
+    uint32_t total = 0;
+    for (int b0 = 0; b0 < upto; b0 += 64) {
+      const Segments q = at(b0);
+      uint32_t t = b0 + lane < upto ? (uint32_t)f(q) * q.blocks * p.G : 0;
+#pragma unroll
+      for (int m = 32; m > 0; m >>= 1) t += __shfl_xor(t, m, 64);
+      total += __builtin_amdgcn_readfirstlane(t);
+    }
+    return total;
+  }
+  __device__ __forceinline__ int run_length() const {
+    const uint32_t total = sum(p.B, [](const Segments& q) { return q.tiles(); });
+    const uint32_t most = p.workgroups - p.B * p.G * p.blocks;      // pieces beyond one a segment
+    return (int)max((uint32_t)RUN, (total + most - 1) / most);
+  }
+};
+
+struct Piece : Segments {
+  int b, g, rb, gs, R, from, to;      // tiles from .. to - 1 of the segment
+  const int* bt;
+  bool whole;
+};
+
+template <int KT, int ROWS>
+__device__ __forceinline__ bool piece_of(const TreeArgs& p, Piece& s, int64_t& part) {
+  int id, j = 0, n = 1;      // piece j of n
+  if (!p.part) {             // row blocks of the same keys are neighbours: one XCD's L2 serves them
+    id = xcd_contiguous(blockIdx.x, p.workgroups);
+    if (id < 0) return false;
+    s.rb = id % p.blocks; s.g = id / p.blocks % p.G; s.b = id / p.blocks / p.G;
+    (Segments&)s = segments_of<KT, ROWS>(p, s.b);
+    if (s.rb >= s.blocks) return false;
+  } else {
+    const Batch<KT, ROWS> all(p);
+    const int run = all.run_length();
+    const uint32_t total = all.sum(p.B, [&](const Segments& q) { return pieces_of(q, run); }), per = (total + 7) >> 3;
+    if ((blockIdx.x >> 3) >= per) return false;
+    id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);      // (the pieces that there are, evenly over the XCDs)
+    if ((uint32_t)id >= total) return false;
+    part = id;
+    bool found = false;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      const Segments q = all.at(b0);
+      const uint32_t t = (uint32_t)pieces_of(q, run) * q.blocks * p.G;
+      uint32_t upto = t;
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) {
+        const uint32_t y = __shfl_up(upto, m, 64);
+        upto += all.lane >= m ? y : 0;
+      }
+      const uint64_t has = __ballot((uint32_t)id < upto);
+      if (has) {
+        const int l = __builtin_ctzll(has);
+        id -= __builtin_amdgcn_readlane(upto - t, l);
+        s.b = b0 + l;
+        s.f0 = __builtin_amdgcn_readlane(q.f0, l); s.drafted = __builtin_amdgcn_readlane(q.drafted, l); s.length = __builtin_amdgcn_readlane(q.length, l);
+        s.t0 = __builtin_amdgcn_readlane(q.t0, l); s.nt = __builtin_amdgcn_readlane(q.nt, l); s.nd = __builtin_amdgcn_readlane(q.nd, l);
+        s.blocks = __builtin_amdgcn_readlane(q.blocks, l);
+        found = true;
+        break;
+      }
+      id -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    if (!found) return false;
+    n = pieces_of(s, run);
+    // row blocks of the same keys are neighbours
+    s.rb = id % s.blocks; id /= s.blocks;
+    j = id % n; s.g = id / n;
+  }
+  s.from = (int)((int64_t)j * s.tiles() / n);
+  s.to = (int)((int64_t)(j + 1) * s.tiles() / n);
+  s.whole = n == 1;
+  // (all of it is uniform; says so where the compiler does not see it)
+  for (int* f : {&s.f0, &s.drafted, &s.length, &s.t0, &s.nt, &s.nd, &s.blocks, &s.b, &s.g, &s.rb, &s.from, &s.to}) *f = __builtin_amdgcn_readfirstlane(*f);
+  part *= ROWS;          // rows of the scratch in front of this piece's
+  s.gs = p.H / p.G;
+  s.R = s.drafted * s.gs;
+  s.bt = p.bt + (int64_t)s.b * p.bt_stride;
+  return true;
+}
+
+// Many rows (lm_tree_wide.hip)
 bool tree_wide_takes(int rows, int dk, int dv);
 int tree_wide_rows(int rows, int dk, int dv);      // of a workgroup
-int launch_tree_wide(TreeArgs& a, int dk, int dv, hipStream_t s);
+int launch_tree_wide(const TreeArgs& a, int dk, int dv, hipStream_t s);
 
 }  // namespace lm

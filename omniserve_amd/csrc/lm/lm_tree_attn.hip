@@ -56,7 +56,7 @@ struct Tree {
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int r = 0; r < 4; ++r) t = fmaxf(t, x[u][r]);
-    t = column_max(t);
+    t = rows_max(t);
     const float m_new = t <= NEG ? m_run[i] : fmaxf(m_run[i], t);
     const float m_sub = (m_new <= NEG ? 0.f : m_new) - SHIFT;
     const float alpha = __builtin_amdgcn_exp2f(m_run[i] - m_new);
@@ -152,12 +152,13 @@ struct Tree {
     f32x4 ev[NU], inv[NU];
     bool bad = false;
     if (edge) {
+      const int k4 = here(4 * l4);
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         uint32_t w = 0;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int key = 16 * u + 4 * l4 + r;
+          const int key = k4 + 16 * u + r;
           w |= (key >= lo && key < hi ? c.vx[u] >> (8 * r) & 255 : 127u) << (8 * r);
         }
         c.vx[u] = w;
@@ -169,9 +170,10 @@ struct Tree {
       for (int r = 0; r < 4; ++r) { ev[u][r] = exponent_of(c.vx[u], r); inv[u][r] = inverse_of(c.vx[u], r); }
     if constexpr (SPLIT) {
       if (edge) {
+        const int first = here(lane / (DV / 16));
 #pragma unroll
         for (int i = 0; i < DV / 16; ++i) {
-          const int row = (64 * i + lane) / (DV / 16);
+          const int row = first + 64 * i / (DV / 16);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             c.v[i][e] = row >= lo && row < hi ? drop_nan_codes(c.v[i][e], bad) : 0u;
@@ -186,7 +188,7 @@ struct Tree {
         *(u32x4*)(stage + row * DV + ((slot ^ code_swizzle<DV>(row)) << 4)) = c.v[i];
       }
     }
-    const int64_t here = c.at;
+    const int64_t page_at = c.at;
     next();
     if constexpr (SPLIT) wave_sync();
     f16x4 pq[NR][NU];
@@ -195,11 +197,17 @@ struct Tree {
 #pragma unroll
       for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float y = __builtin_fmaf(x[i][u][r], p.scale, ev[u][r]);
-          const int key = 16 * u + 4 * l4 + r;
-          x[i][u][r] = !edge || ((int)(key >= lo) & (int)(key < hi) & (int)(kb + key > low[i])) ? y : NEG;
-        }
+        for (int r = 0; r < 4; ++r) x[i][u][r] = __builtin_fmaf(x[i][u][r], p.scale, ev[u][r]);
+      if (edge) {
+        const int k4 = here(4 * l4);
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int key = k4 + 16 * u + r;
+            x[i][u][r] = (int)(key >= lo) & (int)(key < hi) & (int)(kb + key > low[i]) ? x[i][u][r] : NEG;
+          }
+      }
       softmax<NU, false>(i, x[i], inv, 1.f);
       if constexpr (SPLIT) {
 #pragma unroll
@@ -242,7 +250,7 @@ struct Tree {
       bad = __any(bad);
     }
     if (bad) {
-      const uint8_t* vb = p.vc + here * DV;
+      const uint8_t* vb = p.vc + page_at * DV;
       add_nonfinite(lo, min(hi, KT), [&](int i, int j) { return kb + j > low[i]; }, [&](int j, int d) { return (vb[j * DV + d] & 127) == 127 ? __builtin_nanf("") : 0.f; });
     }
   }
@@ -334,10 +342,14 @@ struct Tree {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float y = __builtin_fmaf(x[i][u][r], p.scale, ev);
-          x[i][u][r] = !edge || seen(i, 16 * u + 4 * l4 + r) ? y : NEG;
-        }
+        for (int r = 0; r < 4; ++r) x[i][u][r] = __builtin_fmaf(x[i][u][r], p.scale, ev);
+      if (edge) {
+        const int key = here(4 * l4);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, key + 16 * u + r) ? x[i][u][r] : NEG;
+      }
       softmax<2, true>(i, x[i], x[i], pow2(-e));
 #pragma unroll
       for (int u = 0; u < 2; ++u) split_quad(x[i][u], pq[i][u]);
@@ -379,14 +391,15 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
   typedef Tree<DK, DV, NR, CODES> T;
   __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
   __shared__ float wm[4][16], wl[4][16];
-  Share sh;
-  if (!share_of(p, sh, 16 * NR)) return;
-  const int split = sh.split, g = sh.g, f0 = sh.f0, drafted = sh.drafted, gs = sh.gs, R = sh.R, r0 = sh.rb * 16 * NR, length = sh.length;
-  const int* bt = sh.bt;
+  Piece s;
+  int64_t part = 0;
+  if (!piece_of<T::KT, 16 * NR>(p, s, part)) return;
+  const int g = s.g, f0 = s.f0, drafted = s.drafted, gs = s.gs, R = s.R, r0 = s.rb * 16 * NR, length = s.length;
+  const int* bt = s.bt;
 
   T t(p);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  t.lane = tid & 63; t.l15 = tid & 15; t.l4 = (tid & 63) >> 4;
+  t.lane = tid & 63; t.l15 = tid & 15; t.l4 = t.lane >> 4;
   t.stage = lds + wave * (SPLIT ? T::STAGE : 0);
   int low_min = INT32_MAX, low_max = INT32_MIN, token[NR];
 #pragma unroll
@@ -394,7 +407,7 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
     const int r = r0 + 16 * i + t.l15, rc = min(r, R - 1), tk = rc / gs;
     token[i] = f0 + tk;
     t.row_ok[i] = r < R;
-    const int lo = p.pos[token[i]] - p.window;
+    const int lo = bound_of(p, p.pos[token[i]]);
     low_min = min(low_min, lo);
     low_max = max(low_max, lo);
     t.low[i] = r < R ? lo : INT32_MAX;
@@ -417,8 +430,7 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
   low_max = __builtin_amdgcn_readfirstlane(low_max);
 
   // ---- the context ----
-  const int k0 = max(low_min + 1, 0), t0 = min(k0, length) / T::KT, nt = (length + T::KT - 1) / T::KT - t0;
-  const int per = (nt + p.nsplit - 1) / p.nsplit, ta = t0 + min(split * per, nt), tb = t0 + min((split + 1) * per, nt);
+  const int k0 = max(low_min, -1) + 1, ta = s.t0 + min(s.from, s.nt), tb = s.t0 + min(s.to, s.nt);
   constexpr int PER_PAGE = PAGE / T::KT;
   int tile = ta + wave;
   if (tile < tb) {
@@ -460,9 +472,9 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
       }
     }
   }
-  // ---- the drafted tokens, by the last part: waves that had a tile less come first ----
-  if (split == p.nsplit - 1) {
-    for (int j0 = 32 * ((wave - (tb - ta)) & 3); j0 < drafted; j0 += 128) {
+  // ---- the drafted tokens: waves that had a tile less come first ----
+  if (s.to > s.nt) {
+    for (int j0 = 32 * (max(s.from - s.nt, 0) + ((wave - (tb - ta)) & 3)); j0 < min(drafted, 32 * (s.to - s.nt)); j0 += 128) {
       typename T::Elems c;
       const int64_t row = f0 + j0;
       t.load_elems(c, p.k + row * p.ldk + (int64_t)g * DK, p.ldk, p.v + row * p.ldv + (int64_t)g * DV, p.ldv, min(drafted - j0, 32));
@@ -501,8 +513,8 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
         sum += f * wl[w][rr];
         y += f * *(const f32x4*)&res[w][rr][d];
       }
-      if (p.nsplit > 1) {
-        const int64_t at = ((int64_t)(f0 + tk) * p.H + h) * p.nsplit + split;
+      if (!s.whole) {
+        const int64_t at = part + 16 * i + rr;
         *(f32x4*)(p.part + at * DV + d) = y;
         if (d == 0) { p.ml[2 * at] = m; p.ml[2 * at + 1] = sum; }
       } else {
@@ -513,42 +525,55 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
   }
 }
 
-// Joins the parts: a wave per (token, head), lane s holds the maximum and sum of part s.
-template <int DV>
-__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)p.n * p.H) return;
-  const int tk = (int)(row / p.H), h = (int)(row - (int64_t)tk * p.H);
-  // rows of no sequence, or past its max_draft tokens, were not written
-  int lo = 0, hi = p.B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.first[mid] <= tk) lo = mid;
-    else hi = mid;
-  }
-  if (tk < p.first[lo] || tk >= p.first[lo + 1] || tk - p.first[lo] >= p.max_draft) return;
-  const bool in = lane < p.nsplit;
-  const float ms = in ? p.ml[2 * (row * p.nsplit + lane)] : NEG, ls = in ? p.ml[2 * (row * p.nsplit + lane) + 1] : 0.f;
-  float m = ms;
+// Joins the pieces of a segment's rows: a wave a row, or (few rows, whose pieces are many) all four, a quarter of the pieces each.  Lane s holds the maximum
+// and sum of piece s of 64.
+template <int KT, int ROWS, int DV>
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p, int rows, int waves) {
+  __shared__ float res[3][DV + 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), each = 4 / waves, per = (rows + each - 1) / each;
+  const int seg = blockIdx.x / per, rr = (blockIdx.x - seg * per) * each + (waves == 1 ? wave : 0), w = waves == 1 ? 0 : wave;
+  const int rb = seg % p.blocks, g = seg / p.blocks % p.G, b = seg / p.blocks / p.G, gs = p.H / p.G, r = rb * ROWS + rr;
+  const Batch<KT, ROWS> all(p);
+  const Segments q = segments_of<KT, ROWS>(p, b);
+  const int run = all.run_length(), parts = pieces_of(q, run);
+  if (rr >= ROWS || r >= q.drafted * gs || parts == 1) return;      // (one piece: written by it)
+  const uint32_t before = all.sum(b, [&](const Segments& o) { return pieces_of(o, run); });
+  auto at = [&](int s) { return (before + (int64_t)(g * parts + s) * q.blocks + rb) * ROWS + rr; };
+  float m = NEG;
+  for (int s = lane; s < parts; s += 64) m = fmaxf(m, p.ml[2 * at(s)]);
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
-  const float f = ls != 0.f ? __builtin_amdgcn_exp2f(ms - m) : 0.f, sum = wave_sum(f * ls), inv = sum != 0.f ? 1.0f / sum : 0.f;
-  const float* q = p.part + row * p.nsplit * DV;
-  float y[DV / 64] = {};
-  for (int s0 = 0; s0 < p.nsplit; s0 += 4) {
-    float v[4][DV / 64];
+  float sum = 0.f, y[DV / 64] = {};
+  for (int s0 = 0; s0 < parts; s0 += 64) {
+    const bool in = s0 + lane < parts;
+    const float ms = in ? p.ml[2 * at(s0 + lane)] : NEG, ls = in ? p.ml[2 * at(s0 + lane) + 1] : 0.f;
+    const float f = ls != 0.f ? __builtin_amdgcn_exp2f(ms - m) : 0.f;
+    sum += wave_sum(f * ls);
+    for (int s1 = w; s1 < min(64, parts - s0); s1 += 8 * waves) {
+      float v[8][DV / 64];
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+      for (int s = 0; s < 8; ++s)
 #pragma unroll
-      for (int c = 0; c < DV / 64; ++c) v[s][c] = s0 + s < p.nsplit ? q[(s0 + s) * DV + 64 * c + lane] : 0.f;
+        for (int c = 0; c < DV / 64; ++c) v[s][c] = s0 + s1 + s * waves < parts ? p.part[at(s0 + s1 + s * waves) * DV + 64 * c + lane] : 0.f;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const float w = s0 + s < 64 ? __shfl(f, (s0 + s) & 63, 64) : 0.f;
+      for (int s = 0; s < 8; ++s) {
+        const float u = s1 + s * waves < 64 ? __shfl(f, (s1 + s * waves) & 63, 64) : 0.f;
 #pragma unroll
-      for (int c = 0; c < DV / 64; ++c) y[c] += w != 0.f ? w * v[s][c] : 0.f;      // (an empty part's values are not written; NaN weights pass)
+        for (int c = 0; c < DV / 64; ++c) y[c] += u * v[s][c];
+      }
     }
   }
+  if (waves > 1) {      // (uniform over the workgroup, as are the returns above)
+    if (w > 0)
+#pragma unroll
+      for (int c = 0; c < DV / 64; ++c) res[w - 1][64 * c + lane] = y[c];
+    __syncthreads();
+    if (w > 0) return;
+#pragma unroll
+    for (int c = 0; c < DV / 64; ++c) y[c] += res[0][64 * c + lane] + res[1][64 * c + lane] + res[2][64 * c + lane];
+  }
+  const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+  const int tk = q.f0 + r / gs, h = g * gs + r % gs;
 #pragma unroll
   for (int c = 0; c < DV / 64; ++c) p.o[(int64_t)tk * p.ldo + (int64_t)h * DV + 64 * c + lane] = (elem_t)(y[c] * inv);
 }
@@ -557,48 +582,66 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p) {
 static int row_blocks(int rows) { return rows <= 16 || !SPLIT ? 1 : 2; }
 
 template <int DK, int DV, bool CODES>
-static int launch_tree(TreeArgs& a, hipStream_t s) {
-  const int rows = a.max_draft * (a.H / a.G), nr = row_blocks(rows);
-  a.blocks = (rows + 16 * nr - 1) / (16 * nr);
-  const int64_t groups = (int64_t)a.B * a.G * a.nsplit * a.blocks;
-  if (groups > 1 << 28) return LM_EINVAL;
-  const dim3 grid((unsigned)((groups + 7) / 8 * 8));
+static int launch_tree(const TreeArgs& a, int nr, hipStream_t s) {
+  const dim3 grid((a.workgroups + 7) / 8 * 8);
   if (nr == 1) hipLaunchKernelGGL((tree_attn_kernel<DK, DV, 1, CODES>), grid, dim3(256), 0, s, a);
   if constexpr (SPLIT && DK <= 128 && DV <= 128)
     if (nr == 2) hipLaunchKernelGGL((tree_attn_kernel<DK, DV, 2, CODES>), grid, dim3(256), 0, s, a);
   return launch_status();
 }
 
+template <int KT, int ROWS>
 static void launch_merge(const TreeArgs& a, int dv, hipStream_t s) {
-  const dim3 grid((unsigned)(((int64_t)a.n * a.H + 3) / 4));
-  if (dv == 64) hipLaunchKernelGGL((tree_merge_kernel<64>), grid, dim3(256), 0, s, a);
-  else if (dv == 128) hipLaunchKernelGGL((tree_merge_kernel<128>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((tree_merge_kernel<256>), grid, dim3(256), 0, s, a);
+  const int rows = min(ROWS, a.max_draft * (a.H / a.G));      // of a segment, at most
+  const int64_t segments = (int64_t)a.B * a.G * a.blocks;
+  const int waves = segments * rows <= 512 ? 4 : 1, each = 4 / waves;
+  const dim3 grid((unsigned)(segments * ((rows + each - 1) / each)));
+  if (dv == 64) hipLaunchKernelGGL((tree_merge_kernel<KT, ROWS, 64>), grid, dim3(256), 0, s, a, rows, waves);
+  else if (dv == 128) hipLaunchKernelGGL((tree_merge_kernel<KT, ROWS, 128>), grid, dim3(256), 0, s, a, rows, waves);
+  else hipLaunchKernelGGL((tree_merge_kernel<KT, ROWS, 256>), grid, dim3(256), 0, s, a, rows, waves);
+}
+
+struct Plan {
+  bool wide, cut;
+  int each, kt, blocks;       // rows of a workgroup; keys of a tile
+  int64_t workgroups, scratch;
+};
+#ifndef FINE
+#define FINE 1
+#endif
+// Cut where the segments are fewer than four rounds of workgroups and the longest has more than a run
+static Plan plan_of(int B, int max_draft, int max_context, int H, int G, int dk, int dv, bool codes) {
+  Plan q{};
+  const int rows = max_draft * (H / G);
+  q.wide = tree_wide_takes(rows, dk, dv);
+  q.each = q.wide ? tree_wide_rows(rows, dk, dv) : 16 * row_blocks(rows);
+  q.kt = codes ? 64 : 32;
+  q.blocks = (rows + q.each - 1) / q.each;
+  const int64_t segments = (int64_t)B * G * q.blocks, tiles = max_context / q.kt + (max_context % q.kt > 0) + (max_draft + 31) / 32;
+  const int64_t fit = q.wide ? 256 * 256 / q.each : 512;      // two waves a SIMD
+  q.cut = tiles > RUN && segments < 4 * fit;
+  q.workgroups = q.cut ? segments + min(FINE * fit, (segments * tiles + RUN - 1) / RUN) : segments;
+  q.scratch = q.cut ? q.workgroups * q.each * (dv + 2) : 0;
+  return q;
 }
 
 }  // namespace lm
 
 using namespace lm;
 
-// Enough workgroups for two waves a SIMD, parts of at least eight tiles
-extern "C" int lm_tree_attn_splits(int B, int max_draft, int max_context, int H, int G, int dk, int dv) {
-  if (B <= 0 || G <= 0 || H <= 0 || H % G || max_draft <= 0) return 1;
-  const int rows = max_draft * (H / G);
-  const bool wide = tree_wide_takes(rows, dk, dv);
-  const int each = wide ? tree_wide_rows(rows, dk, dv) : 16 * row_blocks(rows);
-  const int64_t groups = (int64_t)B * G * ((rows + each - 1) / each), fill = wide ? 256 * 256 / each : 512;
-  const int tiles = max_context / 64 + (max_context % 64 > 0);
-  const int64_t want = (fill + groups - 1) / groups;
-  return (int)max((int64_t)1, min(min(want, (int64_t)(tiles + 7) / 8), (int64_t)64));
+extern "C" int64_t lm_tree_attn_scratch(int B, int max_draft, int max_context, int H, int G, int dk, int dv, int codes) {
+  if (B <= 0 || G <= 0 || H <= 0 || H % G || max_draft <= 0 || max_context < 0 || (int64_t)max_draft * H > 1 << 24) return 0;
+  return plan_of(B, max_draft, max_context, H, G, dk, dv, codes != 0).scratch;
 }
 
 extern "C" int lm_tree_attn(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, const void* kc, const void* vc, const uint8_t* ke,
                             const uint8_t* ve, int64_t pages, const int* bt, int bt_stride, int bt_width, const int* length, const int* first, const int* pos,
-                            const int64_t* mask, int words, void* o, int64_t ldo, float* part, int nsplit, float scale, int window, int B, int n, int max_draft,
-                            int H, int G, int dk, int dv, void* stream) {
+                            const int64_t* mask, int words, void* o, int64_t ldo, float* part, float scale, int window, int B, int n, int max_draft,
+                            int max_context, int H, int G, int dk, int dv, void* stream) {
   if (B < 0 || n < 0 || max_draft < 0 || G <= 0 || H <= 0 || H % G || !(scale > 0.f) || window <= 0 || words < 0 || bt_width < 0 || bt_stride < bt_width ||
-      bt_width > INT32_MAX / PAGE || pages < 0 || pages > INT32_MAX / PAGE || (bt_width > 0 && pages == 0) || nsplit < 1 || nsplit > 64 || (nsplit > 1 && !part) ||
-      (ke == nullptr) != (ve == nullptr) || ldq % FR || ldk % FR || ldv % FR || ldo % 4 || (int64_t)max_draft * H > 1 << 24)
+      bt_width > INT32_MAX / PAGE || pages < 0 || pages > INT32_MAX / PAGE || (bt_width > 0 && pages == 0) || max_context < 0 || (ke == nullptr) != (ve == nullptr) || ldq % FR || ldk % FR || ldv % FR || ldo % 4 || (int64_t)max_draft * H > 1 << 24 ||
+      // (tiles are counted in 32 bits)
+      (int64_t)B * G * (max_draft * (H / G) / 16 + 1) * (2 * (int64_t)bt_width + max_draft / 32 + 2) > INT32_MAX)
     return LM_EINVAL;
   if (B == 0 || n == 0 || max_draft == 0) return LM_OK;
   if (!q || !k || !v || !length || !first || !pos || !mask || !o || (bt_width > 0 && (!bt || !kc || !vc)) ||
@@ -609,16 +652,25 @@ extern "C" int lm_tree_attn(const void* q, int64_t ldq, const void* k, int64_t l
   a.kc = (const uint8_t*)kc; a.vc = (const uint8_t*)vc; a.ke = ke; a.ve = ve; a.pages = (int)pages;
   a.bt = bt; a.bt_stride = bt_stride; a.bt_width = bt_width; a.length = length; a.first = first; a.pos = pos;
   a.mask = (const unsigned long long*)mask; a.words = words; a.o = (elem_t*)o; a.ldo = ldo;
-  a.part = part; a.ml = part ? part + (int64_t)n * H * nsplit * dv : nullptr;
-  a.scale = scale * LOG2E; a.window = window; a.n = n; a.H = H; a.G = G; a.B = B; a.nsplit = nsplit; a.max_draft = max_draft;
+  a.scale = scale * LOG2E; a.window = window; a.n = n; a.H = H; a.G = G; a.B = B; a.max_draft = max_draft;
+  Plan plan = plan_of(B, max_draft, max_context, H, G, dk, dv, ke != nullptr);
+  if (!part && plan.cut) { plan.cut = false; plan.workgroups = (int64_t)B * G * plan.blocks; }
+  a.blocks = plan.blocks;
+  a.workgroups = (int)plan.workgroups;
+  if (plan.cut) { a.part = part; a.ml = part + plan.workgroups * plan.each * dv; }
   hipStream_t s = (hipStream_t)stream;
   int rc = LM_EINVAL;
-  if (tree_wide_takes(max_draft * (H / G), dk, dv)) rc = launch_tree_wide(a, dk, dv, s);
-#define LM_CASE(K, V) else if (dk == K && dv == V) rc = ke ? launch_tree<K, V, true>(a, s) : launch_tree<K, V, false>(a, s);
+  if (plan.wide) rc = launch_tree_wide(a, dk, dv, s);
+#define LM_CASE(K, V) else if (dk == K && dv == V) rc = ke ? launch_tree<K, V, true>(a, plan.each / 16, s) : launch_tree<K, V, false>(a, plan.each / 16, s);
   LM_CASE(64, 64) LM_CASE(64, 128) LM_CASE(64, 256) LM_CASE(128, 64) LM_CASE(128, 128) LM_CASE(128, 256)
   LM_CASE(256, 64) LM_CASE(256, 128) LM_CASE(256, 256)
 #undef LM_CASE
   if (rc != LM_OK) return rc;
-  if (nsplit > 1) launch_merge(a, dv, s);
+  if (plan.cut) {
+#define LM_CASE(KT, ROWS) if (plan.kt == KT && plan.each == ROWS) launch_merge<KT, ROWS>(a, dv, s);
+    LM_CASE(64, 16) LM_CASE(64, 32) LM_CASE(64, 64) LM_CASE(64, 128) LM_CASE(64, 256)
+    LM_CASE(32, 16) LM_CASE(32, 32) LM_CASE(32, 64) LM_CASE(32, 128) LM_CASE(32, 256)
+#undef LM_CASE
+  }
   return launch_status();
 }

@@ -49,8 +49,9 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   typedef Wide<DK, DV, NW, CODES> W;
   constexpr int NR = W::NR, NU = W::NU, NVB = W::NVB, KT = W::KT;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  Share s;
-  if (!share_of(p, s, W::ROWS)) return;
+  Piece s;
+  int64_t part = 0;
+  if (!piece_of<KT, W::ROWS>(p, s, part)) return;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l15 = lane & 15, l4 = lane >> 4;
   uint8_t* own = lds + W::NBUF * W::SLOT + wave * W::OWN;
   int* shared = (int*)(lds + W::NBUF * W::SLOT + NW * W::OWN);      // smallest, largest of the rows' bounds; a tile's largest value, whether it has non-finite ones
@@ -67,7 +68,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   int low[NR], low_min = INT32_MAX, low_max = INT32_MIN;
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
-    const int lo = p.pos[token_of(i)] - p.window;
+    const int lo = bound_of(p, p.pos[token_of(i)]);
     low_min = min(low_min, lo);
     low_max = max(low_max, lo);
     low[i] = row_ok(i) ? lo : INT32_MAX;
@@ -83,8 +84,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   __syncthreads();
   low_min = __builtin_amdgcn_readfirstlane(shared[0]);
   low_max = __builtin_amdgcn_readfirstlane(shared[1]);
-  const int k0 = max(low_min + 1, 0), t0 = min(k0, s.length) / KT, nt = (s.length + KT - 1) / KT - t0;
-  const int per = (nt + p.nsplit - 1) / p.nsplit, ta = t0 + min(s.split * per, nt), tb = t0 + min((s.split + 1) * per, nt);
+  const int k0 = max(low_min, -1) + 1, ta = s.t0 + min(s.from, s.nt), tb = s.t0 + min(s.to, s.nt);
 
   // ---- the ring ----
   // Offsets of this lane's pieces: place in the slot -> byte of the tile in memory
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int r = 0; r < 4; ++r) t = fmaxf(t, x[u][r]);
-    t = column_max(t);
+    t = rows_max(t);
     const float m_new = t <= NEG ? m_run[i] : fmaxf(m_run[i], t * p.scale);
     const float m_sub = (m_new <= NEG ? 0.f : m_new) - W::SHIFT;
     const float alpha = __builtin_amdgcn_exp2f(m_run[i] - m_new);
@@ -240,10 +240,11 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       if (edge) {
+        const int key = here(4 * l4);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, 16 * u + 4 * l4 + r) ? x[i][u][r] : NEG;
+          for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, key + 16 * u + r) ? x[i][u][r] : NEG;
       }
       softmax(i, x[i], x[i], Yes(), pow2(-e));
 #pragma unroll
@@ -396,10 +397,11 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
           if (edge) {
+            const int key = here(4 * l4);
 #pragma unroll
             for (int u = 0; u < NU; ++u)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, 16 * u + 4 * l4 + r) ? x[i][u][r] : NEG;
+              for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, key + 16 * u + r) ? x[i][u][r] : NEG;
           }
           softmax(i, x[i], inv, No(), 1.f);
 #pragma unroll
@@ -424,8 +426,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
     }
   }
 
-  // ---- the drafted tokens: the last part ----
-  if (s.split == p.nsplit - 1) {
+  // ---- the drafted tokens ----
+  if (s.to > s.nt) {
     typedef Wide<DK, DV, NW, false> E;      // 32 keys of elements in the ring's memory
     frag_t q[NR][DK / 32];
 #pragma unroll
@@ -434,7 +436,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
       for (int k = 0; k < DK / 32; ++k) q[i][k] = row_ok(i) ? *(const frag_t*)(qrow + 32 * k + 8 * l4) : frag_t{};
     }
-    for (int j0 = 0; j0 < s.drafted; j0 += 32) {
+    for (int j0 = 32 * max(s.from - s.nt, 0); j0 < min(s.drafted, 32 * (s.to - s.nt)); j0 += 32) {
       const int rows = min(s.drafted - j0, 32);
       const int64_t row0 = s.f0 + j0;
       uint8_t* kt = lds;
@@ -471,8 +473,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
     const float l = column_sum(l_run[i]);
     if (!row_ok(i)) continue;
     const int r = r0 + 16 * i + l15, tk = r / s.gs, h = s.g * s.gs + r - tk * s.gs;
-    if (p.nsplit > 1) {
-      const int64_t at = ((int64_t)(s.f0 + tk) * p.H + h) * p.nsplit + s.split;
+    if (!s.whole) {
+      const int64_t at = part + wave * 16 * NR + 16 * i + l15;
 #pragma unroll
       for (int c = 0; c < NVB; ++c) *(f32x4*)(p.part + at * DV + 16 * c + 4 * l4) = acc[i][c];
       if (l4 == 0) { p.ml[2 * at] = m_run[i]; p.ml[2 * at + 1] = l; }
@@ -485,17 +487,12 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 }
 
 template <int DK, int DV, int NW, bool CODES>
-static int launch(TreeArgs& a, hipStream_t s) {
+static int launch(const TreeArgs& a, hipStream_t s) {
   typedef Wide<DK, DV, NW, CODES> W;
-  const int rows = a.max_draft * (a.H / a.G);
-  a.blocks = (rows + W::ROWS - 1) / W::ROWS;
-  const int64_t groups = (int64_t)a.B * a.G * a.nsplit * a.blocks;
-  if (groups > 1 << 28) return LM_EINVAL;
-  constexpr int E = 32 * 2 * (DK + DV);      // a drafted tile
+  static_assert(W::NBUF * W::SLOT >= 32 * 2 * (DK + DV), "a drafted tile fits the ring");
   constexpr size_t bytes = W::LDS;
-  static_assert(W::NBUF * W::SLOT >= E, "a drafted tile fits the ring");
   if (allow_lds(tree_wide_kernel<DK, DV, NW, CODES>, bytes) != LM_OK) return LM_EINVAL;
-  hipLaunchKernelGGL((tree_wide_kernel<DK, DV, NW, CODES>), dim3((unsigned)((groups + 7) / 8 * 8)), dim3(64 * NW), bytes, s, a);
+  hipLaunchKernelGGL((tree_wide_kernel<DK, DV, NW, CODES>), dim3((a.workgroups + 7) / 8 * 8), dim3(64 * NW), bytes, s, a);
   return launch_status();
 }
 
@@ -508,7 +505,7 @@ static int waves(int rows, int dk, int dv) {
 bool tree_wide_takes(int rows, int dk, int dv) { return rows > 16 * row_blocks(dk, dv); }
 int tree_wide_rows(int rows, int dk, int dv) { return waves(rows, dk, dv) * 16 * row_blocks(dk, dv); }
 
-int launch_tree_wide(TreeArgs& a, int dk, int dv, hipStream_t s) {
+int launch_tree_wide(const TreeArgs& a, int dk, int dv, hipStream_t s) {
   const int nw = waves(a.max_draft * (a.H / a.G), dk, dv);
   const bool codes = a.ke != nullptr;
 #define LM_CASE(K, V)                                                                               \
@@ -526,7 +523,7 @@ int launch_tree_wide(TreeArgs& a, int dk, int dv, hipStream_t s) {
 // f32, the format of verification, has the one kernel
 bool tree_wide_takes(int, int, int) { return false; }
 int tree_wide_rows(int, int, int) { return 1; }
-int launch_tree_wide(TreeArgs&, int, int, hipStream_t) { return LM_EINVAL; }
+int launch_tree_wide(const TreeArgs&, int, int, hipStream_t) { return LM_EINVAL; }
 #endif
 
 }  // namespace lm

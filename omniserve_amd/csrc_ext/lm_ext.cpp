@@ -23,7 +23,7 @@ typedef std::optional<T> OptT;
 typedef std::vector<T> Pools;
 
 constexpr int64_t PAGE = 64;
-constexpr int NO_WINDOW = 1 << 30;
+constexpr int NO_WINDOW = INT32_MAX;
 
 template <typename... What>
 inline void need(bool ok, const What&... what) {
@@ -60,7 +60,7 @@ class Ops {
   decltype(&lm_rope) rope_;
   decltype(&lm_kv_store) store_;
   decltype(&lm_kv_load) load_;
-  decltype(&lm_tree_attn_splits) splits_;
+  decltype(&lm_tree_attn_scratch) scratch_;
   decltype(&lm_tree_attn) tree_;
 
   // a matrix of at least `width` neighbouring columns, and of `n` rows (< 0: of any number)
@@ -106,9 +106,9 @@ class Ops {
   }
 
  public:
-  Ops(bool bf16, uintptr_t rope, uintptr_t store, uintptr_t load, uintptr_t splits, uintptr_t tree)
+  Ops(bool bf16, uintptr_t rope, uintptr_t store, uintptr_t load, uintptr_t scratch, uintptr_t tree)
       : elem(bf16 ? torch::kBFloat16 : torch::kFloat32), rope_((decltype(rope_))rope), store_((decltype(store_))store), load_((decltype(load_))load),
-        splits_((decltype(splits_))splits), tree_((decltype(tree_))tree) {}
+        scratch_((decltype(scratch_))scratch), tree_((decltype(tree_))tree) {}
 
   T rope(const T& x, const OptT& freq, const OptT& pos, int64_t heads, int64_t dk, const std::string& pairing, double factor, const OptT& out) const {
     need(heads > 0 && dk > 0 && heads <= INT32_MAX && dk <= INT32_MAX, "heads of at least one dimension");
@@ -196,12 +196,12 @@ class Ops {
     const c10::DeviceGuard guard(q.device());
     const T o = out ? *out : torch::empty({n, H * s.dv}, q.options());
     const int draft = narrow(max_draft), context = (int)std::min<int64_t>(max_context, INT32_MAX), heads = narrow(H), kv_heads = narrow(s.G), seqs = narrow(B);
-    const int nsplit = splits_(seqs, draft, context, heads, kv_heads, (int)s.dk, (int)s.dv);
-    const T part = nsplit > 1 ? torch::empty({n * H * nsplit * (s.dv + 2)}, q.options().dtype(torch::kFloat32)) : T();
+    const int64_t room = scratch_(seqs, draft, context, heads, kv_heads, (int)s.dk, (int)s.dv, codes);
+    const T part = room ? torch::empty({room}, q.options().dtype(torch::kFloat32)) : T();
     done(tree_(q.data_ptr(), step(q), k.data_ptr(), step(k), v.data_ptr(), step(v), cache[0].data_ptr(), cache[1].data_ptr(), codes ? cache[2].data_ptr<uint8_t>() : nullptr,
                codes ? cache[3].data_ptr<uint8_t>() : nullptr, s.pages, bt.data_ptr<int>(), narrow(B > 1 ? bt.stride(0) : bt.size(1)), narrow(bt.size(1)), length.data_ptr<int>(),
-               first.data_ptr<int>(), pos.data_ptr<int>(), mask.data_ptr<int64_t>(), narrow(mask.size(1)), o.data_ptr(), step(o), nsplit > 1 ? part.data_ptr<float>() : nullptr, nsplit,
-               (float)scale, (int)std::min<int64_t>(window.value_or(NO_WINDOW), NO_WINDOW), seqs, narrow(n), draft, heads, kv_heads, (int)s.dk, (int)s.dv, stream(q)),
+               first.data_ptr<int>(), pos.data_ptr<int>(), mask.data_ptr<int64_t>(), narrow(mask.size(1)), o.data_ptr(), step(o), room ? part.data_ptr<float>() : nullptr,
+               (float)scale, (int)std::min<int64_t>(window.value_or(NO_WINDOW), NO_WINDOW), seqs, narrow(n), draft, context, heads, kv_heads, (int)s.dk, (int)s.dv, stream(q)),
          "lm_tree_attn");
     return o;
   }

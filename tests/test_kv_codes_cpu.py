@@ -153,18 +153,23 @@ def test_library_refuses(ops):
     assert h.lm_kv_load(64, 64, 64, 64, 64, 64, 64, 64, 3, 64, 0, 1, 64, 64, None) == 0
     assert h.lm_kv_load(64, 64, 64, 64, 64, 64, 64, 64, 3, None, 1, 1, 64, 64, None) == -22
     assert h.lm_kv_load(64, 65, 64, 64, 64, 64, 64, 64, 3, 64, 1, 1, 64, 64, None) == -22
-    tree = lambda B=1, n=1, draft=1, H=2, G=1, dk=64, dv=64, width=2, pages=3, splits=1, part=None, scale=f, window=1, ldq=128, ke=64, ve=64, q=64: h.lm_tree_attn(      # noqa: E731
-        q, ldq, 64, 64, 64, 64, 64, 64, ke, ve, pages, 64, width, width, 64, 64, 64, 64, 1, 64, 128, part, splits, scale, window, B, n, draft, H, G, dk, dv, None)
+    tree = lambda B=1, n=1, draft=1, H=2, G=1, dk=64, dv=64, width=2, pages=3, context=100, scale=f, window=1, ldq=128, ke=64, ve=64, q=64: h.lm_tree_attn(      # noqa: E731
+        q, ldq, 64, 64, 64, 64, 64, 64, ke, ve, pages, 64, width, width, 64, 64, 64, 64, 1, 64, 128, None, scale, window, B, n, draft, context, H, G, dk, dv, None)
     assert tree(B=0) == tree(n=0) == tree(draft=0) == 0
-    for bad in (dict(H=3, G=2), dict(dk=80), dict(dv=192), dict(pages=0), dict(splits=0), dict(splits=65, part=64), dict(splits=2), dict(scale=0.0), dict(scale=float("nan")), dict(window=0),
+    for bad in (dict(H=3, G=2), dict(dk=80), dict(dv=192), dict(pages=0), dict(context=-1), dict(width=1 << 26, pages=1 << 20), dict(scale=0.0), dict(scale=float("nan")), dict(window=0),
                 dict(ldq=129), dict(ke=None), dict(ve=None), dict(q=None), dict(q=72), dict(B=-1)):
         assert tree(**bad) == -22, bad
 
 
-def test_parts_of_the_keys(ops):
-    """Parts for few workgroups and long contexts, none where there are enough or too few keys, never more than the kernel joins"""
-    s = ops._h.lm_tree_attn_splits
-    assert s(1, 1, 0, 32, 8, 128, 128) == 1 and s(1, 1, 64, 32, 8, 128, 128) == 1
-    assert 1 < s(1, 1, 100000, 32, 8, 128, 128) <= 64 and s(1, 1, 2 ** 31 - 1, 1, 1, 128, 128) == 64
-    assert s(512, 1, 100000, 32, 8, 128, 128) == 1
-    assert s(0, 1, 100, 32, 8, 128, 128) == s(1, 0, 100, 32, 8, 128, 128) == s(1, 1, 100, 3, 2, 128, 128) == 1
+def test_scratch_of_cut_keys(ops):
+    """Room for pieces of the keys where workgroups are few and contexts long; none for short contexts and for batches that fill the chip several times; no
+    more than the pieces there can be"""
+    room = ops._h.lm_tree_attn_scratch
+    for codes in (0, 1):
+        assert room(1, 1, 0, 32, 8, 128, 128, codes) == 0 and room(1, 1, 64, 32, 8, 128, 128, codes) == 0
+        assert room(1, 1, 100000, 32, 8, 128, 128, codes) > 0 and room(1, 1, 2 ** 31 - 1, 1, 1, 128, 128, codes) > 0
+        assert room(512, 1, 100000, 32, 8, 128, 128, codes) == 0
+        # few keys: pieces of four tiles, one more a segment (a tile is 64 keys of codes, 32 of elements; one of drafted tokens)
+        tiles = 8 * (2000 // (64 if codes else 32) + 1 + 1)
+        assert room(1, 1, 2000, 32, 8, 128, 128, codes) == (8 + tiles // 4) * 16 * 130
+    assert room(0, 1, 10000, 32, 8, 128, 128, 1) == room(1, 0, 10000, 32, 8, 128, 128, 1) == room(1, 1, 10000, 3, 2, 128, 128, 1) == room(1, 1, -1, 32, 8, 128, 128, 1) == 0
