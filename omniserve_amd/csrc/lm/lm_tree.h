@@ -21,9 +21,11 @@ struct TreeArgs {
   const unsigned long long* mask; int words;
   elem_t* o; int64_t ldo;
   float* ml; float* part;                            // of cut pieces: [workgroups][rows][2] and [workgroups][rows][dv]; null: nothing is cut
+  int* cuts;                                         // [B * G * blocks][2]: a segment's first piece and how many it has
   float scale;                                       // includes log2(e)
   int window;                                        // NO_WINDOW: none
   int n, H, G, B, max_draft, blocks, workgroups;     // blocks: of rows, the most a sequence has
+  int target;                                        // pieces that there should be
 };
 constexpr int NO_WINDOW = INT32_MAX;
 
@@ -140,10 +142,17 @@ struct Batch {
     }
     return total;
   }
+  // The shortest that makes no more pieces than `target` (a piece more than places is a round more), looked for between total / target and three times
+  // that, a length per lane; where none does (more segments than `target`), total / target: at most `target` pieces beyond one a segment.
   __device__ __forceinline__ int run_length() const {
     const uint32_t total = sum(p.B, [](const Segments& q) { return q.tiles(); });
-    const uint32_t most = p.workgroups - p.B * p.G * p.blocks;      // pieces beyond one a segment
-    return (int)max((uint32_t)RUN, (total + most - 1) / most);
+    const uint32_t least = max((uint32_t)RUN, (total + p.target - 1) / p.target);
+    if (p.B > 64) return (int)least;
+    const uint32_t run = least + least * lane / 32, each = mine.tiles(), many = mine.blocks * p.G;
+    uint32_t count = 0;
+    for (int b = 0; b < p.B; ++b) count += (__builtin_amdgcn_readlane(each, b) + run - 1) / run * __builtin_amdgcn_readlane(many, b);
+    const uint64_t fits = __ballot(count <= (uint32_t)p.target);
+    return (int)(fits ? __builtin_amdgcn_readlane(run, __builtin_ctzll(fits)) : least);
   }
 };
 
@@ -198,6 +207,10 @@ __device__ __forceinline__ bool piece_of(const TreeArgs& p, Piece& s, int64_t& p
     // row blocks of the same keys are neighbours
     s.rb = id % s.blocks; id /= s.blocks;
     j = id % n; s.g = id / n;
+    if (j == 0 && threadIdx.x == 0) {
+      int* c = p.cuts + 2 * ((s.b * p.G + s.g) * p.blocks + s.rb);
+      c[0] = (int)part; c[1] = n;      // (its pieces are s.blocks apart)
+    }
   }
   s.from = (int)((int64_t)j * s.tiles() / n);
   s.to = (int)((int64_t)(j + 1) * s.tiles() / n);
@@ -213,6 +226,7 @@ __device__ __forceinline__ bool piece_of(const TreeArgs& p, Piece& s, int64_t& p
 
 // Many rows (lm_tree_wide.hip)
 bool tree_wide_takes(int rows, int dk, int dv);
+int tree_wide_fit(int rows, int dk, int dv, bool codes);      // workgroups on the chip
 int tree_wide_rows(int rows, int dk, int dv);      // of a workgroup
 int launch_tree_wide(const TreeArgs& a, int dk, int dv, hipStream_t s);
 

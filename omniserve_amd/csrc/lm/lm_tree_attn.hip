@@ -527,40 +527,41 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
 
 // Joins the pieces of a segment's rows: a wave a row, or (few rows, whose pieces are many) all four, a quarter of the pieces each.  Lane s holds the maximum
 // and sum of piece s of 64.
-template <int KT, int ROWS, int DV>
+template <int ROWS, int DV>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p, int rows, int waves) {
   __shared__ float res[3][DV + 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), each = 4 / waves, per = (rows + each - 1) / each;
   const int seg = blockIdx.x / per, rr = (blockIdx.x - seg * per) * each + (waves == 1 ? wave : 0), w = waves == 1 ? 0 : wave;
   const int rb = seg % p.blocks, g = seg / p.blocks % p.G, b = seg / p.blocks / p.G, gs = p.H / p.G, r = rb * ROWS + rr;
-  const Batch<KT, ROWS> all(p);
-  const Segments q = segments_of<KT, ROWS>(p, b);
-  const int run = all.run_length(), parts = pieces_of(q, run);
-  if (rr >= ROWS || r >= q.drafted * gs || parts == 1) return;      // (one piece: written by it)
-  const uint32_t before = all.sum(b, [&](const Segments& o) { return pieces_of(o, run); });
-  auto at = [&](int s) { return (before + (int64_t)(g * parts + s) * q.blocks + rb) * ROWS + rr; };
+  const int f0 = min(max(p.first[b], 0), p.n), drafted = min(max(p.first[b + 1] - f0, 0), min(p.max_draft, p.n - f0)), parts = p.cuts[2 * seg + 1];
+  if (rr >= ROWS || r >= drafted * gs || parts == 1) return;      // (one piece: written by it)
+  const int64_t at0 = (int64_t)p.cuts[2 * seg] * ROWS + rr, step = (int64_t)((drafted * gs + ROWS - 1) / ROWS) * ROWS;
   float m = NEG;
-  for (int s = lane; s < parts; s += 64) m = fmaxf(m, p.ml[2 * at(s)]);
+  for (int s = lane; s < parts; s += 64) m = fmaxf(m, p.ml[2 * (at0 + s * step)]);
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
   float sum = 0.f, y[DV / 64] = {};
   for (int s0 = 0; s0 < parts; s0 += 64) {
-    const bool in = s0 + lane < parts;
-    const float ms = in ? p.ml[2 * at(s0 + lane)] : NEG, ls = in ? p.ml[2 * at(s0 + lane) + 1] : 0.f;
-    const float f = ls != 0.f ? __builtin_amdgcn_exp2f(ms - m) : 0.f;
-    sum += wave_sum(f * ls);
-    for (int s1 = w; s1 < min(64, parts - s0); s1 += 8 * waves) {
-      float v[8][DV / 64];
+    float v[8][DV / 64];
+    auto load = [&](int s1) {
 #pragma unroll
       for (int s = 0; s < 8; ++s)
 #pragma unroll
-        for (int c = 0; c < DV / 64; ++c) v[s][c] = s0 + s1 + s * waves < parts ? p.part[at(s0 + s1 + s * waves) * DV + 64 * c + lane] : 0.f;
+        for (int c = 0; c < DV / 64; ++c) v[s][c] = s0 + s1 + s * waves < parts ? p.part[(at0 + (s0 + s1 + s * waves) * step) * DV + 64 * c + lane] : 0.f;
+    };
+    load(w);      // (beside the sums' request)
+    const bool in = s0 + lane < parts;
+    const float ms = in ? p.ml[2 * (at0 + (s0 + lane) * step)] : NEG, ls = in ? p.ml[2 * (at0 + (s0 + lane) * step) + 1] : 0.f;
+    const float f = ls != 0.f ? __builtin_amdgcn_exp2f(ms - m) : 0.f;
+    sum += wave_sum(f * ls);
+    for (int s1 = w; s1 < min(64, parts - s0); s1 += 8 * waves) {
 #pragma unroll
       for (int s = 0; s < 8; ++s) {
         const float u = s1 + s * waves < 64 ? __shfl(f, (s1 + s * waves) & 63, 64) : 0.f;
 #pragma unroll
         for (int c = 0; c < DV / 64; ++c) y[c] += u * v[s][c];
       }
+      if (s1 + 8 * waves < min(64, parts - s0)) load(s1 + 8 * waves);
     }
   }
   if (waves > 1) {      // (uniform over the workgroup, as are the returns above)
@@ -573,7 +574,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p, int rows, i
     for (int c = 0; c < DV / 64; ++c) y[c] += res[0][64 * c + lane] + res[1][64 * c + lane] + res[2][64 * c + lane];
   }
   const float inv = sum != 0.f ? 1.0f / sum : 0.f;
-  const int tk = q.f0 + r / gs, h = g * gs + r % gs;
+  const int tk = f0 + r / gs, h = g * gs + r % gs;
 #pragma unroll
   for (int c = 0; c < DV / 64; ++c) p.o[(int64_t)tk * p.ldo + (int64_t)h * DV + 64 * c + lane] = (elem_t)(y[c] * inv);
 }
@@ -590,38 +591,36 @@ static int launch_tree(const TreeArgs& a, int nr, hipStream_t s) {
   return launch_status();
 }
 
-template <int KT, int ROWS>
+template <int ROWS>
 static void launch_merge(const TreeArgs& a, int dv, hipStream_t s) {
   const int rows = min(ROWS, a.max_draft * (a.H / a.G));      // of a segment, at most
   const int64_t segments = (int64_t)a.B * a.G * a.blocks;
   const int waves = segments * rows <= 512 ? 4 : 1, each = 4 / waves;
   const dim3 grid((unsigned)(segments * ((rows + each - 1) / each)));
-  if (dv == 64) hipLaunchKernelGGL((tree_merge_kernel<KT, ROWS, 64>), grid, dim3(256), 0, s, a, rows, waves);
-  else if (dv == 128) hipLaunchKernelGGL((tree_merge_kernel<KT, ROWS, 128>), grid, dim3(256), 0, s, a, rows, waves);
-  else hipLaunchKernelGGL((tree_merge_kernel<KT, ROWS, 256>), grid, dim3(256), 0, s, a, rows, waves);
+  if (dv == 64) hipLaunchKernelGGL((tree_merge_kernel<ROWS, 64>), grid, dim3(256), 0, s, a, rows, waves);
+  else if (dv == 128) hipLaunchKernelGGL((tree_merge_kernel<ROWS, 128>), grid, dim3(256), 0, s, a, rows, waves);
+  else hipLaunchKernelGGL((tree_merge_kernel<ROWS, 256>), grid, dim3(256), 0, s, a, rows, waves);
 }
 
 struct Plan {
   bool wide, cut;
-  int each, kt, blocks;       // rows of a workgroup; keys of a tile
-  int64_t workgroups, scratch;
+  int each;                   // rows of a workgroup
+  int64_t blocks, workgroups, target, scratch;
 };
-#ifndef FINE
-#define FINE 1
-#endif
-// Cut where the segments are fewer than four rounds of workgroups and the longest has more than a run
+// Cut where the segments are fewer than four rounds of workgroups and the longest has more than a run: into as many pieces as workgroups fit the chip, or
+// twice as many where the segments alone are half of that.
 static Plan plan_of(int B, int max_draft, int max_context, int H, int G, int dk, int dv, bool codes) {
   Plan q{};
-  const int rows = max_draft * (H / G);
+  const int rows = max_draft * (H / G), kt = codes ? 64 : 32;
   q.wide = tree_wide_takes(rows, dk, dv);
   q.each = q.wide ? tree_wide_rows(rows, dk, dv) : 16 * row_blocks(rows);
-  q.kt = codes ? 64 : 32;
   q.blocks = (rows + q.each - 1) / q.each;
-  const int64_t segments = (int64_t)B * G * q.blocks, tiles = max_context / q.kt + (max_context % q.kt > 0) + (max_draft + 31) / 32;
-  const int64_t fit = q.wide ? 256 * 256 / q.each : 512;      // two waves a SIMD
+  const int64_t segments = (int64_t)B * G * q.blocks, tiles = max_context / kt + (max_context % kt > 0) + (max_draft + 31) / 32;
+  const int64_t fit = q.wide ? tree_wide_fit(rows, dk, dv, codes) : dk + dv <= 256 ? 512 : 256;
   q.cut = tiles > RUN && segments < 4 * fit;
-  q.workgroups = q.cut ? segments + min(FINE * fit, (segments * tiles + RUN - 1) / RUN) : segments;
-  q.scratch = q.cut ? q.workgroups * q.each * (dv + 2) : 0;
+  q.target = min(segments > fit / 2 ? 2 * fit : fit, (segments * tiles + RUN - 1) / RUN);
+  q.workgroups = q.cut ? segments + q.target : segments;
+  q.scratch = q.cut ? q.workgroups * q.each * (dv + 2) + 2 * segments : 0;
   return q;
 }
 
@@ -655,9 +654,10 @@ extern "C" int lm_tree_attn(const void* q, int64_t ldq, const void* k, int64_t l
   a.scale = scale * LOG2E; a.window = window; a.n = n; a.H = H; a.G = G; a.B = B; a.max_draft = max_draft;
   Plan plan = plan_of(B, max_draft, max_context, H, G, dk, dv, ke != nullptr);
   if (!part && plan.cut) { plan.cut = false; plan.workgroups = (int64_t)B * G * plan.blocks; }
-  a.blocks = plan.blocks;
+  a.blocks = (int)plan.blocks;
   a.workgroups = (int)plan.workgroups;
-  if (plan.cut) { a.part = part; a.ml = part + plan.workgroups * plan.each * dv; }
+  a.target = (int)plan.target;
+  if (plan.cut) { a.part = part; a.ml = part + plan.workgroups * plan.each * dv; a.cuts = (int*)(a.ml + plan.workgroups * plan.each * 2); }
   hipStream_t s = (hipStream_t)stream;
   int rc = LM_EINVAL;
   if (plan.wide) rc = launch_tree_wide(a, dk, dv, s);
@@ -667,9 +667,8 @@ extern "C" int lm_tree_attn(const void* q, int64_t ldq, const void* k, int64_t l
 #undef LM_CASE
   if (rc != LM_OK) return rc;
   if (plan.cut) {
-#define LM_CASE(KT, ROWS) if (plan.kt == KT && plan.each == ROWS) launch_merge<KT, ROWS>(a, dv, s);
-    LM_CASE(64, 16) LM_CASE(64, 32) LM_CASE(64, 64) LM_CASE(64, 128) LM_CASE(64, 256)
-    LM_CASE(32, 16) LM_CASE(32, 32) LM_CASE(32, 64) LM_CASE(32, 128) LM_CASE(32, 256)
+#define LM_CASE(ROWS) if (plan.each == ROWS) launch_merge<ROWS>(a, dv, s);
+    LM_CASE(16) LM_CASE(32) LM_CASE(64) LM_CASE(128) LM_CASE(256)
 #undef LM_CASE
   }
   return launch_status();

@@ -499,11 +499,20 @@ static int launch(const TreeArgs& a, hipStream_t s) {
 // Waves of a workgroup: as few as hold the rows, as many as share a tile
 static int waves(int rows, int dk, int dv) {
   const int per = 16 * row_blocks(dk, dv);
-  return rows <= 2 * per ? 2 : rows <= 4 * per ? 4 : 8;
+#ifndef WAVES_MAX
+#define WAVES_MAX 8
+#endif
+  return rows <= 2 * per ? 2 : rows <= 4 * per ? 4 : WAVES_MAX;
 }
 
 bool tree_wide_takes(int rows, int dk, int dv) { return rows > 16 * row_blocks(dk, dv); }
 int tree_wide_rows(int rows, int dk, int dv) { return waves(rows, dk, dv) * 16 * row_blocks(dk, dv); }
+
+int tree_wide_fit(int rows, int dk, int dv, bool codes) {
+  const int nw = waves(rows, dk, dv), each = codes ? 1 : 2;
+  const int lds = (nw == 2 ? 2 : 3) * ((codes ? 64 : 32) * each * (dk + dv) + (codes ? 128 : 0)) + (codes ? 512 * nw : 0) + 64;      // (Wide::LDS)
+  return 256 * min(8 / nw, 160 * 1024 / lds);      // two waves a SIMD
+}
 
 int launch_tree_wide(const TreeArgs& a, int dk, int dv, hipStream_t s) {
   const int nw = waves(a.max_draft * (a.H / a.G), dk, dv);
@@ -523,6 +532,7 @@ int launch_tree_wide(const TreeArgs& a, int dk, int dv, hipStream_t s) {
 // f32, the format of verification, has the one kernel
 bool tree_wide_takes(int, int, int) { return false; }
 int tree_wide_rows(int, int, int) { return 1; }
+int tree_wide_fit(int, int, int, bool) { return 1; }
 int launch_tree_wide(const TreeArgs&, int, int, hipStream_t) { return LM_EINVAL; }
 #endif
 
