@@ -100,7 +100,7 @@ __device__ __forceinline__ void rope_heads(const RopeArgs& p, const CosSin<float
           a[u][e] = (elem_t)__builtin_fmaf(y, c, -z * s);
           b[u][e] = (elem_t)__builtin_fmaf(z, c, y * s);
         }
-        if constexpr (VEC) *(frag_t*)(dst[u] + cd[u]) = b[u];
+        if constexpr (VEC) __builtin_nontemporal_store(b[u], (frag_t*)(dst[u] + cd[u]));
         else dst[u][cd[u]] = b[u][0];
       } else if (cd[u] == 0) {
 #pragma unroll
@@ -110,7 +110,7 @@ __device__ __forceinline__ void rope_heads(const RopeArgs& p, const CosSin<float
           a[u][e + 1] = (elem_t)__builtin_fmaf(z, c, y * s);
         }
       }
-      if constexpr (VEC) *(frag_t*)dst[u] = a[u];
+      if constexpr (VEC) __builtin_nontemporal_store(a[u], (frag_t*)dst[u]);
       else {
         dst[u][0] = a[u][0];
         if (cd[u] == 0) dst[u][1] = a[u][1];
@@ -242,61 +242,50 @@ struct LoadArgs {
   const int* slot;
   int64_t places;
   int G, size[2];
-  uint32_t total;                         // pieces of 16 codes of a workgroup's tokens
   int tokens, per;
   Divisor row, piece[2];                  // pieces of a token's keys and values; of one head's key, value
 };
 
-// 16 codes a thread: 16 bytes in, 32 (bf16) out
+// 16 codes a thread: 16 bytes in, 32 (bf16) out; a piece each (several requests a thread, or streamed stores, took 135 - 160 us for 100000 tokens of 8
+// heads, this 125: 4.9 TB/s read and written)
 __global__ __launch_bounds__(256) void kv_load_kernel(LoadArgs p) {
-  constexpr int U = 4;
   const int t0 = blockIdx.x * p.per, n = min(p.per, p.tokens - t0);
   const uint32_t total = (uint32_t)n * p.row.d, keys = (uint32_t)p.G * p.piece[0].d;
-  for (uint32_t i0 = threadIdx.x; i0 < total; i0 += 256 * U) {
-    u32x4 w[U];
-    float f[U];
-    elem_t* dst[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t i = i0 + 256 * u;
-      dst[u] = nullptr;
-      if (i >= total) continue;
-      const int t = p.row.quotient(i);
-      uint32_t j = i - t * p.row.d;
-      const int v = j >= keys;
-      j -= v ? keys : 0;
-      const Divisor& pc = p.piece[v];
-      const int g = pc.quotient(j), c = j - g * pc.d, slot = p.slot[t0 + t];
-      dst[u] = p.out[v] + (int64_t)(t0 + t) * p.ld[v] + (int64_t)g * p.size[v] + 16 * c;
-      w[u] = (u32x4){0, 0, 0, 0};
-      f[u] = 1.f;
-      if (slot < 0 || slot >= p.places) continue;
+  for (uint32_t i = threadIdx.x; i < total; i += 256) {
+    const int t = p.row.quotient(i);
+    uint32_t j = i - t * p.row.d;
+    const int v = j >= keys;
+    j -= v ? keys : 0;
+    const Divisor& pc = p.piece[v];
+    const int g = pc.quotient(j), c = j - g * pc.d, slot = p.slot[t0 + t];
+    u32x4 w = {0, 0, 0, 0};
+    float f = 1.f;
+    if (slot >= 0 && slot < p.places) {
       const int64_t at = ((int64_t)(slot / PAGE) * p.G + g) * PAGE + slot % PAGE;
-      w[u] = *(const u32x4*)(p.codes[v] + at * p.size[v] + 16 * c);
-      f[u] = scale_of(p.exps[v][at]);
+      w = *(const u32x4*)(p.codes[v] + at * p.size[v] + 16 * c);
+      f = scale_of(p.exps[v][at]);
     }
+    elem_t* dst = p.out[v] + (int64_t)(t0 + t) * p.ld[v] + (int64_t)g * p.size[v] + 16 * c;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (!dst[u]) continue;
+    for (int k = 0; k < 16 / FR; ++k) {
+      frag_t y;
 #pragma unroll
-      for (int k = 0; k < 16 / FR; ++k) {
-        frag_t y;
+      for (int m = 0; m < FR / 4; ++m) {
+        const quad_t z = decode4(w[k * (FR / 4) + m], f);
 #pragma unroll
-        for (int m = 0; m < FR / 4; ++m) {
-          const quad_t z = decode4(w[u][k * (FR / 4) + m], f[u]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[4 * m + e] = z[e];
-        }
-        *(frag_t*)(dst[u] + k * FR) = y;
+        for (int e = 0; e < 4; ++e) y[4 * m + e] = z[e];
       }
+      *(frag_t*)(dst + k * FR) = y;
     }
   }
 }
 
 constexpr int MOST_PAIRS = 512, MOST_HEADS = 4096;      // of a head; of a row
 
-// Tokens of a workgroup: enough 16-byte pieces for its 256 threads, no more tokens than leave every CU a few workgroups
-static int tokens_per_group(int tokens) { return tokens >= 4096 ? 4 : tokens >= 1024 ? 2 : 1; }
+// Tokens of a workgroup: four pieces a thread where that leaves a thousand workgroups (12001 tokens of 40 heads: 2 tokens 40 us, 1 43.5, 4 41.4)
+static int tokens_per_group(int tokens, int pieces, int half) {
+  return max(1, min(min((1024 + pieces - 1) / max(pieces, 1), tokens / 1024), min(16, 2048 / max(half, 1))));
+}
 
 // How many heads a workgroup takes: all of them unless tokens are few
 static int heads_per_group(int tokens, int heads) { return tokens >= 512 ? heads : tokens >= 64 ? min(heads, 16) : min(heads, 8); }
@@ -310,13 +299,13 @@ static RopeArgs rope_args(const void* x, int64_t ldx, void* o, int64_t ldo, cons
   a.turn = t;
   a.x = (const elem_t*)x; a.ldx = ldx; a.o = (elem_t*)o; a.ldo = ldo;
   a.tokens = tokens; a.heads = heads; a.dk = dk;
-  a.per = tokens_per_group(tokens);
   a.hpb = heads_per_group(tokens, heads);
   const int turning = t.halves ? t.half : 2 * t.half;      // elements of the pieces that turn
   a.vec = aligned(x, ldx) && aligned(o, ldo) && dk % FR == 0 && turning % FR == 0 && (dk - 2 * t.half) % FR == 0;
   const bool in_place = o == x && ldo == ldx;
   const int rest = in_place ? 0 : dk - 2 * t.half;
   a.items = Divisor(a.vec ? (turning + rest) / FR : t.half + rest);
+  a.per = tokens_per_group(tokens, a.hpb * a.items.d, t.half);
   a.wg_items = Divisor(a.hpb);
   a.half = Divisor(t.half > 0 ? t.half : 1);
   return a;
@@ -350,7 +339,10 @@ extern "C" int lm_kv_store(const void* x, int64_t ldx, int x_rows, const int* ro
   if (tokens == 0) return LM_OK;
   StoreArgs a{};
   a.q = rope_args(x, ldx, q, ldq, Turn{freq, pos, half, halves, factor}, tokens, H > 0 ? H : 1, dk);
-  if (!q) a.q.vec = aligned(x, ldx);
+  if (!q) {
+    a.q.vec = aligned(x, ldx);
+    a.q.per = tokens_per_group(tokens, G * (dk + dv) / FR, half);
+  }
   a.rows = rows; a.x_rows = x_rows; a.slot = slot;
   a.kc = kc; a.vc = vc; a.ke = ke; a.ve = ve; a.places = pages * PAGE;
   a.H = H; a.G = G; a.dk = dk; a.dv = dv;
@@ -376,8 +368,7 @@ extern "C" int lm_kv_load(void* k, int64_t ldk, void* v, int64_t ldv, const uint
   a.tokens = tokens;
   a.row = Divisor(G * (dk + dv) / 16);
   a.piece[0] = Divisor(dk / 16); a.piece[1] = Divisor(dv / 16);
-  a.per = tokens >= 4096 ? 8 : tokens >= 1024 ? 4 : 1;
-  if ((int64_t)a.per * a.row.d * a.row.d >= 1ll << 32) a.per = 1;
+  a.per = max(1u, 256 / a.row.d);
   if ((int64_t)a.row.d * a.row.d >= 1ll << 32) return LM_EINVAL;
   hipLaunchKernelGGL(kv_load_kernel, dim3((tokens + a.per - 1) / a.per), dim3(256), 0, (hipStream_t)stream, a);
   return launch_status();

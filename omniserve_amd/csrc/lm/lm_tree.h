@@ -25,7 +25,7 @@ struct TreeArgs {
   float scale;                                       // includes log2(e)
   int window;                                        // NO_WINDOW: none
   int n, H, G, B, max_draft, blocks, workgroups;     // blocks: of rows, the most a sequence has
-  int target;                                        // pieces that there should be
+  int target, run;                                   // pieces that there should be; tiles of one at least
 };
 constexpr int NO_WINDOW = INT32_MAX;
 
@@ -90,7 +90,6 @@ __device__ __forceinline__ uint32_t drop_nan_codes(uint32_t w, bool& bad) {
 // the tiles of all of them, so that there are as many pieces as suit the chip whatever the sequences' lengths are (a fixed number of parts a sequence
 // leaves the short ones' places idle).  A segment of one piece is written by it, others are joined by tree_merge_kernel.  The division depends on the
 // lengths alone.
-constexpr int RUN = 4;      // tiles of a piece at least, where it is not all of its segment (for each of the narrow kernel's waves one)
 
 struct Segments {            // of one sequence
   int f0, drafted, length, t0, nt, nd, blocks;
@@ -146,12 +145,15 @@ struct Batch {
   // that, a length per lane; where none does (more segments than `target`), total / target: at most `target` pieces beyond one a segment.
   __device__ __forceinline__ int run_length() const {
     const uint32_t total = sum(p.B, [](const Segments& q) { return q.tiles(); });
-    const uint32_t least = max((uint32_t)RUN, (total + p.target - 1) / p.target);
+    const uint32_t least = max((uint32_t)p.run, (total + p.target - 1) / p.target);
     if (p.B > 64) return (int)least;
-    const uint32_t run = least + least * lane / 32, each = mine.tiles(), many = mine.blocks * p.G;
-    uint32_t count = 0;
-    for (int b = 0; b < p.B; ++b) count += (__builtin_amdgcn_readlane(each, b) + run - 1) / run * __builtin_amdgcn_readlane(many, b);
-    const uint64_t fits = __ballot(count <= (uint32_t)p.target);
+    // (counted in f32: a length that makes a piece more than it seems is as good)
+    const uint32_t run = least + least * lane / 32;
+    const float each = (float)mine.tiles(), many = (float)(mine.blocks * p.G), inv = 1.0f / (float)run;
+    float count = 0.f;
+    for (int b = 0; b < p.B; ++b)
+      count = __builtin_fmaf(ceilf(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(each), b)) * inv), __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(many), b)), count);
+    const uint64_t fits = __ballot(count <= (float)p.target);
     return (int)(fits ? __builtin_amdgcn_readlane(run, __builtin_ctzll(fits)) : least);
   }
 };

@@ -29,7 +29,8 @@ struct Tree {
   static constexpr int CH = DK / 64, PF = 16 / FR, NKF = CH * PF, NVB = DV / 16;
   static constexpr int KT = CODES ? 64 : 32, NU = KT / 16;        // keys of a context tile
   static constexpr int STAGE = 64 * DV;                           // bytes of a wave's V tile: 64 rows of codes, 32 of bf16
-  static constexpr int RED = 4 * 16 * (DV + 4) * 4, LDS = SPLIT && 4 * STAGE > RED ? 4 * STAGE : RED;
+  static constexpr int NW = 4;                                    // waves
+  static constexpr int RED = NW * 16 * (DV + 4) * 4, LDS = SPLIT && NW * STAGE > RED ? NW * STAGE : RED;
   typedef Tile<SPLIT ? DV * 2 : 256> VT;
 
   const TreeArgs& p;
@@ -390,7 +391,8 @@ template <int DK, int DV, int NR, bool CODES>
 __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_attn_kernel(TreeArgs p) {
   typedef Tree<DK, DV, NR, CODES> T;
   __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
-  __shared__ float wm[4][16], wl[4][16];
+  constexpr int NW = T::NW;
+  __shared__ float wm[NW][16], wl[NW][16];
   Piece s;
   int64_t part = 0;
   if (!piece_of<T::KT, 16 * NR>(p, s, part)) return;
@@ -438,15 +440,15 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
     if constexpr (CODES) {
       typename T::Codes c;
       t.load_codes(c, page, g);
-      int ahead = tile + 4 < tb ? bt[tile + 4] : 0;
-      for (; tile < tb; tile += 4) {
+      int ahead = tile + NW < tb ? bt[tile + NW] : 0;
+      for (; tile < tb; tile += NW) {
         const int kb = tile * T::KT, hi = (uint32_t)page < (uint32_t)p.pages ? length - kb : 0;
         const bool edge = hi < T::KT || kb <= low_max;
         page = ahead;
         t.code_tile(c, kb, max(k0 - kb, 0), hi, edge, [&]() {
-          if (tile + 4 >= tb) return;
+          if (tile + NW >= tb) return;
           t.load_codes(c, page, g);
-          ahead = tile + 8 < tb ? bt[tile + 8] : 0;
+          ahead = tile + 2 * NW < tb ? bt[tile + 2 * NW] : 0;
         });
       }
     } else {
@@ -458,23 +460,23 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
         t.load_elems(c, kc + at * DK, DK, vc + at * DV, DV, T::KT);
       };
       load(tile, page);
-      int ahead = tile + 4 < tb ? bt[(tile + 4) / PER_PAGE] : 0;
-      for (; tile < tb; tile += 4) {
+      int ahead = tile + NW < tb ? bt[(tile + NW) / PER_PAGE] : 0;
+      for (; tile < tb; tile += NW) {
         const int kb = tile * T::KT, hi = (uint32_t)page < (uint32_t)p.pages ? length - kb : 0, lo = max(k0 - kb, 0);
         const bool edge = hi < T::KT || kb <= low_max;
         page = ahead;
         t.elem_tile(c, lo, hi, edge, [&](int i, int key) { return (bool)((int)(key >= lo) & (int)(key < hi) & (int)(kb + key > t.low[i])); },
                     [&]() {
-                      if (tile + 4 >= tb) return;
-                      load(tile + 4, page);
-                      ahead = tile + 8 < tb ? bt[(tile + 8) / PER_PAGE] : 0;
+                      if (tile + NW >= tb) return;
+                      load(tile + NW, page);
+                      ahead = tile + 2 * NW < tb ? bt[(tile + 2 * NW) / PER_PAGE] : 0;
                     });
       }
     }
   }
   // ---- the drafted tokens: waves that had a tile less come first ----
   if (s.to > s.nt) {
-    for (int j0 = 32 * (max(s.from - s.nt, 0) + ((wave - (tb - ta)) & 3)); j0 < min(drafted, 32 * (s.to - s.nt)); j0 += 128) {
+    for (int j0 = 32 * (max(s.from - s.nt, 0) + ((wave - (tb - ta)) & (NW - 1))); j0 < min(drafted, 32 * (s.to - s.nt)); j0 += 32 * NW) {
       typename T::Elems c;
       const int64_t row = f0 + j0;
       t.load_elems(c, p.k + row * p.ldk + (int64_t)g * DK, p.ldk, p.v + row * p.ldv + (int64_t)g * DV, p.ldv, min(drafted - j0, 32));
@@ -502,13 +504,15 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
     if (t.l4 == 0) { wm[wave][t.l15] = t.m_run[i]; wl[wave][t.l15] = l; }
     __syncthreads();
     const int rows = min(16, R - r0 - 16 * i);
-    for (int at = tid; at < rows * (DV / 4); at += 256) {
+    for (int at = tid; at < rows * (DV / 4); at += 64 * NW) {
       const int rr = at / (DV / 4), d = (at - rr * (DV / 4)) * 4, r = r0 + 16 * i + rr, tk = r / gs, h = g * gs + r - tk * gs;
-      const float m = fmaxf(fmaxf(wm[0][rr], wm[1][rr]), fmaxf(wm[2][rr], wm[3][rr]));
+      float m = wm[0][rr];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) m = fmaxf(m, wm[w][rr]);
       f32x4 y = zero4();
       float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < NW; ++w) {
         const float f = wl[w][rr] != 0.f ? __builtin_amdgcn_exp2f(wm[w][rr] - m) : 0.f;
         sum += f * wl[w][rr];
         y += f * *(const f32x4*)&res[w][rr][d];
@@ -605,10 +609,12 @@ static void launch_merge(const TreeArgs& a, int dv, hipStream_t s) {
 struct Plan {
   bool wide, cut;
   int each;                   // rows of a workgroup
-  int64_t blocks, workgroups, target, scratch;
+  int64_t run, blocks, workgroups, target, scratch;
 };
-// Cut where the segments are fewer than four rounds of workgroups and the longest has more than a run: into as many pieces as workgroups fit the chip, or
-// twice as many where the segments alone are half of that.
+// Cut where the segments are fewer than four rounds of workgroups and the longest has more tiles than joining is worth: a workgroup of the narrow kernel
+// takes 20 in the 10 us that it costs to join, one of the wide kernel 8 (one token, 1501 keys of 8 heads in one piece each 17.2 us, in pieces of 4 tiles
+// 14.9; 16 of 1024 keys 17.1 and 20.2; a tree of 26, 500 keys @w).  Into as many pieces as workgroups fit the chip, or twice as many where the segments alone
+// are half of that (61 tokens of 300 - 4000 keys @n).
 static Plan plan_of(int B, int max_draft, int max_context, int H, int G, int dk, int dv, bool codes) {
   Plan q{};
   const int rows = max_draft * (H / G), kt = codes ? 64 : 32;
@@ -616,9 +622,10 @@ static Plan plan_of(int B, int max_draft, int max_context, int H, int G, int dk,
   q.each = q.wide ? tree_wide_rows(rows, dk, dv) : 16 * row_blocks(rows);
   q.blocks = (rows + q.each - 1) / q.each;
   const int64_t segments = (int64_t)B * G * q.blocks, tiles = max_context / kt + (max_context % kt > 0) + (max_draft + 31) / 32;
-  const int64_t fit = q.wide ? tree_wide_fit(rows, dk, dv, codes) : dk + dv <= 256 ? 512 : 256;
-  q.cut = tiles > RUN && segments < 4 * fit;
-  q.target = min(segments > fit / 2 ? 2 * fit : fit, (segments * tiles + RUN - 1) / RUN);
+  const int64_t fit = q.wide ? tree_wide_fit(rows, dk, dv, codes) : q.each == 16 && dk + dv <= 256 ? 512 : 256;
+  q.run = q.wide ? 3 : 4;
+  q.cut = tiles > (q.wide ? 8 : 20) && segments < 4 * fit;
+  q.target = min(segments > fit / 2 ? 2 * fit : fit, (segments * tiles + q.run - 1) / q.run);
   q.workgroups = q.cut ? segments + q.target : segments;
   q.scratch = q.cut ? q.workgroups * q.each * (dv + 2) + 2 * segments : 0;
   return q;
@@ -657,6 +664,7 @@ extern "C" int lm_tree_attn(const void* q, int64_t ldq, const void* k, int64_t l
   a.blocks = (int)plan.blocks;
   a.workgroups = (int)plan.workgroups;
   a.target = (int)plan.target;
+  a.run = (int)plan.run;
   if (plan.cut) { a.part = part; a.ml = part + plan.workgroups * plan.each * dv; a.cuts = (int*)(a.ml + plan.workgroups * plan.each * 2); }
   hipStream_t s = (hipStream_t)stream;
   int rc = LM_EINVAL;

@@ -24,6 +24,10 @@ __device__ __forceinline__ int key_swizzle(int row) {
   else return Tile<ROWB>::swizzle(row);
 }
 
+// A row's weights are relative to a maximum that is followed only when it has grown by so much (in powers of two): what has been added up is rescaled in a
+// few tiles, not in every second one
+constexpr float LAZY = 8.f;
+
 // Blocks of 16 rows of a wave: what 256 registers hold
 constexpr int row_blocks(int dk, int dv) { return dk > 128 || dv > 128 ? 1 : 2; }
 
@@ -39,7 +43,7 @@ struct Wide {
   static constexpr int OWN = CODES ? 512 : 0;                                     // a wave's: keys' exponents
   static constexpr int LDS = NBUF * SLOT + NW * OWN + 64;
   static constexpr int KS = CODES ? (DK + 127) / 128 : DK / 32;                  // steps of a key's product
-  static constexpr float SHIFT = CODES ? 14.f : 0.f;
+  static constexpr float SHIFT = CODES ? 7.f : 0.f;                              // weights of codes are f16: at most 2^(LAZY + 7)
   typedef Tile<2 * DV> VT;
   typedef Tile<2 * DK> KTile;
 };
@@ -58,33 +62,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   const int r0 = s.rb * W::ROWS + wave * 16 * NR;
   const bool live = r0 < s.R;                                         // (a wave without rows fetches its pieces and waits with the others)
 
-  // ---- rows ----
-  auto token_of = [&](int i) { return s.f0 + min(r0 + 16 * i + l15, s.R - 1) / s.gs; };
-  auto query_of = [&](int i) {
-    const int tk = token_of(i);
-    return p.q + (int64_t)tk * p.ldq + (int64_t)(s.g * s.gs + min(r0 + 16 * i + l15, s.R - 1) - (tk - s.f0) * s.gs) * DK;
-  };
-  auto row_ok = [&](int i) { return r0 + 16 * i + l15 < s.R; };
-  int low[NR], low_min = INT32_MAX, low_max = INT32_MIN;
-#pragma unroll
-  for (int i = 0; i < NR; ++i) {
-    const int lo = bound_of(p, p.pos[token_of(i)]);
-    low_min = min(low_min, lo);
-    low_max = max(low_max, lo);
-    low[i] = row_ok(i) ? lo : INT32_MAX;
-  }
-  if (tid == 0) { shared[0] = INT32_MAX; shared[1] = INT32_MIN; }
-  __syncthreads();
-#pragma unroll
-  for (int m = 1; m < 16; m <<= 1) {
-    low_min = min(low_min, __shfl_xor(low_min, m, 64));
-    low_max = max(low_max, __shfl_xor(low_max, m, 64));
-  }
-  if (lane == 0) { atomicMin(&shared[0], low_min); atomicMax(&shared[1], low_max); }
-  __syncthreads();
-  low_min = __builtin_amdgcn_readfirstlane(shared[0]);
-  low_max = __builtin_amdgcn_readfirstlane(shared[1]);
-  const int k0 = max(low_min, -1) + 1, ta = s.t0 + min(s.from, s.nt), tb = s.t0 + min(s.to, s.nt);
+  const int ta = s.t0 + min(s.from, s.nt), tb = s.t0 + min(s.to, s.nt);
 
   // ---- the ring ----
   // Offsets of this lane's pieces: place in the slot -> byte of the tile in memory
@@ -121,6 +99,34 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
   for (int j = 0; j < W::NBUF - 1; ++j)
     if (ta + j < tb) fetch(ta + j, pages[j], j);
+
+  // ---- rows ----
+  auto token_of = [&](int i) { return s.f0 + min(r0 + 16 * i + l15, s.R - 1) / s.gs; };
+  auto query_of = [&](int i) {
+    const int tk = token_of(i);
+    return p.q + (int64_t)tk * p.ldq + (int64_t)(s.g * s.gs + min(r0 + 16 * i + l15, s.R - 1) - (tk - s.f0) * s.gs) * DK;
+  };
+  auto row_ok = [&](int i) { return r0 + 16 * i + l15 < s.R; };
+  int low[NR], low_min = INT32_MAX, low_max = INT32_MIN;
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int lo = bound_of(p, p.pos[token_of(i)]);
+    low_min = min(low_min, lo);
+    low_max = max(low_max, lo);
+    low[i] = row_ok(i) ? lo : INT32_MAX;
+  }
+  if (tid == 0) { shared[0] = INT32_MAX; shared[1] = INT32_MIN; }
+  __syncthreads();
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) {
+    low_min = min(low_min, __shfl_xor(low_min, m, 64));
+    low_max = max(low_max, __shfl_xor(low_max, m, 64));
+  }
+  if (lane == 0) { atomicMin(&shared[0], low_min); atomicMax(&shared[1], low_max); }
+  __syncthreads();
+  low_min = __builtin_amdgcn_readfirstlane(shared[0]);
+  low_max = __builtin_amdgcn_readfirstlane(shared[1]);
+  const int k0 = max(low_min, -1) + 1;
 
   // ---- queries ----
   i32x8 qc[NR][2][CODES ? W::KS : 1];      // codes: hi, lo
@@ -187,9 +193,9 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) t = fmaxf(t, x[u][r]);
     t = rows_max(t);
-    const float m_new = t <= NEG ? m_run[i] : fmaxf(m_run[i], t * p.scale);
-    const float m_sub = (m_new <= NEG ? 0.f : m_new) - W::SHIFT;
-    const float alpha = __builtin_amdgcn_exp2f(m_run[i] - m_new);
+    t = t <= NEG ? NEG : t * p.scale;
+    const bool grows = t > m_run[i] + LAZY;      // (the first key's always; a NaN never)
+    const float m_new = grows ? t : m_run[i], m_sub = (m_new <= NEG ? 0.f : m_new) - W::SHIFT;
     float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -199,12 +205,14 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
         if constexpr (one.value) sum += x[u][r];
         else sum = __builtin_fmaf(x[u][r], inv[u][r], sum);
       }
-    l_run[i] = __builtin_fmaf(l_run[i], alpha, one.value ? sum * inv_all : sum);
-    m_run[i] = m_new;
-    if (__any(alpha != 1.0f)) {
+    if (__any(grows)) {
+      const float alpha = __builtin_amdgcn_exp2f(m_run[i] - m_new);
+      l_run[i] *= alpha;
 #pragma unroll
       for (int c = 0; c < NVB; ++c) acc[i][c] *= alpha;
     }
+    l_run[i] += one.value ? sum * inv_all : sum;
+    m_run[i] = m_new;
   };
   auto wave_sync = [&]() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -499,10 +507,7 @@ static int launch(const TreeArgs& a, hipStream_t s) {
 // Waves of a workgroup: as few as hold the rows, as many as share a tile
 static int waves(int rows, int dk, int dv) {
   const int per = 16 * row_blocks(dk, dv);
-#ifndef WAVES_MAX
-#define WAVES_MAX 8
-#endif
-  return rows <= 2 * per ? 2 : rows <= 4 * per ? 4 : WAVES_MAX;
+  return rows <= 2 * per ? 2 : rows <= 4 * per ? 4 : 8;
 }
 
 bool tree_wide_takes(int rows, int dk, int dv) { return rows > 16 * row_blocks(dk, dv); }

@@ -169,7 +169,7 @@ def test_scratch_of_cut_keys(ops):
         assert room(1, 1, 0, 32, 8, 128, 128, codes) == 0 and room(1, 1, 64, 32, 8, 128, 128, codes) == 0
         assert room(1, 1, 100000, 32, 8, 128, 128, codes) > 0 and room(1, 1, 2 ** 31 - 1, 1, 1, 128, 128, codes) > 0
         assert room(512, 1, 100000, 32, 8, 128, 128, codes) == 0
-        # few keys: pieces of four tiles, one more a segment (a tile is 64 keys of codes, 32 of elements; one of drafted tokens)
+        # few keys: pieces of four tiles, one more a segment (a tile is 64 keys of codes, 32 of elements; one of drafted tokens), and where each segment is cut
         tiles = 8 * (2000 // (64 if codes else 32) + 1 + 1)
-        assert room(1, 1, 2000, 32, 8, 128, 128, codes) == (8 + tiles // 4) * 16 * 130
+        assert room(1, 1, 2000, 32, 8, 128, 128, codes) == (8 + tiles // 4) * 16 * 130 + 2 * 8
     assert room(0, 1, 10000, 32, 8, 128, 128, 1) == room(1, 0, 10000, 32, 8, 128, 128, 1) == room(1, 1, 10000, 3, 2, 128, 128, 1) == room(1, 1, -1, 32, 8, 128, 128, 1) == 0
