@@ -271,46 +271,27 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       for (int i = 0; i < NR; ++i) add_nonfinite(i, lo, hi, seen, value);
     }
   };
-  // Values of a tile that not every row sees: rows outside lo .. hi - 1 and non-finite ones become zero; elements are divided by 2^e (codes' kernel).
-  // -> whether there were non-finite ones
-  auto clean_elems = [&](uint8_t* vt, int lo, int hi, int& e) {
-    if (tid == 0) { shared[2] = 0; shared[3] = 0; }
+  // Values of a tile of elements that not every row sees: rows outside lo .. hi - 1 and non-finite ones become zero -> whether there were non-finite ones
+  auto clean_elems = [&](uint8_t* vt, int lo, int hi) {
+    if (tid == 0) shared[2] = 0;
     __syncthreads();
     bool bad = false;
-    float top = 0.f;
     for (int i = tid; i < 32 * DV / 8; i += 64 * NW) {
       const int row = i / (DV / 8);
       frag_t* at = (frag_t*)(vt + W::VT::slot(row, i % (DV / 8)));
       frag_t f = *at;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        float y = row >= lo && row < hi ? (float)f[k] : 0.f;
+        const float y = row >= lo && row < hi ? (float)f[k] : 0.f;
         const bool fine = fabsf(y) < __builtin_inff();
         bad |= !fine;
-        y = fine ? y : 0.f;
-        top = fmaxf(top, fabsf(y));
-        f[k] = (elem_t)y;
+        f[k] = (elem_t)(fine ? y : 0.f);
       }
       *at = f;
     }
     if (bad) atomicOr(&shared[2], 1);
-    atomicMax(&shared[3], (int)__float_as_uint(top));      // (not negative: ordered like whole numbers)
     __syncthreads();
-    bad = shared[2] != 0;
-    e = 0;
-    if constexpr (CODES) {
-      e = row_exponent(__uint_as_float((uint32_t)shared[3]));
-      const float f = pow2(-e);
-      for (int i = tid; i < 32 * DV / 8; i += 64 * NW) {
-        frag_t* at = (frag_t*)(vt + W::VT::slot(i / (DV / 8), i % (DV / 8)));
-        frag_t y = *at;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] = (elem_t)((float)y[k] * f);
-        *at = y;
-      }
-      __syncthreads();
-    }
-    return bad;
+    return shared[2] != 0;
   };
 
   // ---- the context ----
@@ -332,10 +313,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
     auto seen = [&](int i, int key) { return (bool)((int)(key >= lo) & (int)(key < hi) & (int)(kb + key > low[i])); };
     bool bad = false;
     if constexpr (!CODES) {
-      if (edge) {
-        int e;
-        bad = clean_elems(vt, lo, hi, e);
-      }
+      if (edge) bad = clean_elems(vt, lo, hi);
       if (live) {
         const elem_t* vb = (const elem_t*)p.vc + at * DV;
         elem_products(kt, vt, qf, edge, bad, 0, lo, min(hi, KT), seen, [&](int j, int d) { return (float)vb[j * DV + d]; });
@@ -449,18 +427,51 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       const int64_t row0 = s.f0 + j0;
       uint8_t* kt = lds;
       uint8_t* vt = lds + E::KBYTES;
+      // Values pass through registers: non-finite ones are left out, codes' kernels divide by a power of two
+      constexpr int VF = (32 * DV / 8 + 64 * NW - 1) / (64 * NW);
+      if (tid == 0) { shared[2] = 0; shared[3] = 0; }
+      frag_t vf[VF];
+      bool bad = false;
+      float top = 0.f;
+#pragma unroll
+      for (int k = 0; k < VF; ++k) {
+        const int i = tid + 64 * NW * k, row = i / (DV / 8), c = i % (DV / 8);
+        vf[k] = row < rows ? *(const frag_t*)(p.v + (row0 + row) * p.ldv + (int64_t)s.g * DV + 8 * c) : frag_t{};
+      }
       __syncthreads();      // what was there has been read
       for (int i = tid; i < 32 * DK / 8; i += 64 * NW) {
         const int row = i / (DK / 8), c = i % (DK / 8);
         *(frag_t*)(kt + W::KTile::slot(row, c)) = *(const frag_t*)(p.k + (row0 + min(row, rows - 1)) * p.ldk + (int64_t)s.g * DK + 8 * c);
       }
-      for (int i = tid; i < 32 * DV / 8; i += 64 * NW) {
-        const int row = i / (DV / 8), c = i % (DV / 8);
-        *(frag_t*)(vt + W::VT::slot(row, c)) = *(const frag_t*)(p.v + (row0 + min(row, rows - 1)) * p.ldv + (int64_t)s.g * DV + 8 * c);
+#pragma unroll
+      for (int k = 0; k < VF; ++k)
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+          const float y = (float)vf[k][m];
+          const bool fine = fabsf(y) < __builtin_inff();
+          bad |= !fine;
+          vf[k][m] = fine ? vf[k][m] : (elem_t)0.f;
+          top = fine ? fmaxf(top, fabsf(y)) : top;
+        }
+      if constexpr (CODES) {
+#pragma unroll
+        for (int m = 32; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+        if (lane == 0) atomicMax(&shared[3], (int)__float_as_uint(top));      // (not negative: ordered like whole numbers)
+      }
+      if (__any(bad) && lane == 0) atomicOr(&shared[2], 1);
+      __syncthreads();
+      bad = shared[2] != 0;
+      const int e = CODES ? row_exponent(__uint_as_float((uint32_t)shared[3])) : 0;
+      const float f = pow2(-e);
+#pragma unroll
+      for (int k = 0; k < VF; ++k) {
+        const int i = tid + 64 * NW * k, row = i / (DV / 8), c = i % (DV / 8);
+        if constexpr (CODES)
+#pragma unroll
+          for (int m = 0; m < 8; ++m) vf[k][m] = (elem_t)((float)vf[k][m] * f);
+        if (row < 32) *(frag_t*)(vt + W::VT::slot(row, c)) = vf[k];
       }
       __syncthreads();
-      int e;
-      const bool bad = clean_elems(vt, 0, rows, e);
       if (!live) continue;
       uint32_t bits[NR];
 #pragma unroll

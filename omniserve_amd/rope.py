@@ -5,7 +5,8 @@ reference evaluates on the device (common/decoderMaskedMultiheadAttentionUtils.h
 Building it once on the host (numpy float32) makes the RoPE bit-reproducible and removes
 powf/sincosf from the bandwidth-bound kernels.
 
-`inverse_frequencies` is what the engine's layers use instead: they turn by position * frequency inside the kernel.
+`inverse_frequencies` is what the engine's layers use instead: they turn by position * frequency inside the kernel; it and `stretched_frequencies` are what
+LmOps.rope and kv_store take, as a float64 tensor.
 """
 from __future__ import annotations
 
@@ -32,6 +33,21 @@ def inverse_frequencies(dims: int, base: float, scaling=None) -> list:
                 f = (1.0 - s) * f / scaling["factor"] + s * f
         out.append(f)
     return out
+
+
+def stretched_frequencies(dims: int, base: float, factor: float, original: int, fast: float = 32.0, slow: float = 1.0):
+    """Rotation per position of the dims // 2 pairs (float64) for a context `factor` times the original one, and what cosine and sine are multiplied with
+    (YaRN, Peng et al. 2023): pairs that turn more than `fast` times within the original context keep their frequency, those that turn less than `slow`
+    times are slowed down by factor, between them the two are blended linearly in the pair's number; scores are sharpened by (0.1 ln factor + 1)^2."""
+    if dims < 2 or dims % 2 or not factor >= 1 or not fast > slow > 0:
+        raise ValueError("an even number of dimensions, a factor of at least one and fast > slow > 0")
+    pair = lambda turns: dims * math.log(original / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))      # noqa: E731
+    first, last = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), dims - 1)
+    out = []
+    for i, f in enumerate(inverse_frequencies(dims, base)):
+        keep = 1.0 - min(1.0, max(0.0, (i - first) / max(last - first, 1e-3)))
+        out.append(f * keep + f / factor * (1.0 - keep))
+    return out, 0.1 * math.log(factor) + 1.0
 
 
 _cache = {}

@@ -100,12 +100,12 @@ def attention(q, k, v, mask, first, pos, kpool, vpool, bt, length, scale, window
 def attention_bound(dtype, codes, dk, ref, size, sums, peak, count, coarse):
     """How far lm_tree_attn may be from 64 bits: the result's rounding; then relative to sum p |v|: scores are sums of dk products in f32 (twice that
     for the order, and the conversion to a power of two), whose error enters every p and the total; a weight is 11 bits where values are codes (half a step
-    2^-12, twice for the total's that is not rounded) and 16 of two bf16, or f32; exponentials and f32 sums of all keys.  Weights below 2^-39 of the
-    largest (times its values' power of two, at most 2^-7 of the row's largest value) are lost.  Many rows over codes: a query element is two codes,
+    2^-12, twice for the total's that is not rounded) and 16 of two bf16, or f32; exponentials and f32 sums of all keys.  An f16
+    weight is at least 2^7 for the largest (times its values' power of two, at most 2^-7 of the row's largest value), and off by 2^-25 where it is small: 2^-32 of that.  Many rows over codes: a query element is two codes,
     q = 2^e (hi + lo / 16), max |q| > 224 * 2^e; hi is off by at most half a step, 2^-4 of it or (below 2^-6) 2^-10, lo is 16 times that, at most 256, and off by 2^-10 where it is below
     2^-6 and not at all where its 4 bits hold the rest (bf16 has 8): the element by 2^-14 * 2^e < 2^-21 max |q|; that times |k|, in every p and the total."""
     weight = (2.0 ** -12 if codes else 2.0 ** -16) if dtype == torch.bfloat16 else 2.0 ** -23
     rel = 2 * (dk + 4) * 2.0 ** -24 * (sums + 1.0) + weight + (count + 8) * 2.0 ** -24 + 2.0 ** -21
     rel = rel + (2 * 2.0 ** -21 * coarse if codes and dtype == torch.bfloat16 else 0.0)
-    lost = count * 2.0 ** -39 * peak * 448 / 224 if codes and dtype == torch.bfloat16 else 0.0
+    lost = count * 2.0 ** -32 * peak * 448 / 224 if codes and dtype == torch.bfloat16 else 0.0
     return 1.01 * UNIT[dtype] * ref.abs() + rel * size + lost + 1e-30

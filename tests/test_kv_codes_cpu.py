@@ -44,6 +44,25 @@ def test_empty_pools_hold_zeros():
     assert all(t.dtype == torch.uint8 for t in c) and int(c.k.max()) == 0 and int(c.k_exp.min()) == 27 == int(c.v_exp.max())
 
 
+def test_stretched_frequencies():
+    """Fast pairs as they are, slow ones divided by the factor, no step between, and the known factor of the scores"""
+    import math
+
+    from omniserve_amd.rope import inverse_frequencies, stretched_frequencies
+    for dims, base, factor, original in ((128, 10000.0, 16.0, 4096), (64, 500000.0, 8.0, 8192), (2, 10000.0, 4.0, 2048)):
+        plain, (got, scale) = inverse_frequencies(dims, base), stretched_frequencies(dims, base, factor, original)
+        assert scale == 0.1 * math.log(factor) + 1.0 and len(got) == dims // 2
+        share = [(1.0 - g / f) / (1.0 - 1.0 / factor) for f, g in zip(plain, got)]      # 0: kept, 1: divided
+        turns = [original * f / (2 * math.pi) for f in plain]
+        assert all(-1e-12 <= x <= 1 + 1e-12 for x in share) and share == sorted(share)
+        assert all(abs(x) < 1e-12 for x, t in zip(share, turns) if t >= 32.0 * base ** (2.0 / dims))
+        assert all(abs(x - 1) < 1e-12 for x, t in zip(share, turns) if t <= base ** (-2.0 / dims))
+    assert stretched_frequencies(64, 10000.0, 1.0, 4096)[0] == pytest.approx(inverse_frequencies(64, 10000.0), rel=1e-15) and stretched_frequencies(64, 10000.0, 1.0, 4096)[1] == 1.0
+    for bad in ((3, 10000.0, 2.0, 4096), (0, 10000.0, 2.0, 4096), (64, 10000.0, 0.5, 4096), (64, 10000.0, 2.0, 4096, 1.0, 2.0)):
+        with pytest.raises(ValueError):
+            stretched_frequencies(*bad)
+
+
 def refuse(match, call, *args, **kw):
     with pytest.raises(ValueError, match=match):
         call(*args, **kw)
