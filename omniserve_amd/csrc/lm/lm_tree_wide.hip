@@ -158,14 +158,16 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       for (int k = 0; k < W::KS; ++k)
 #pragma unroll
         for (int w = 0; w < 8; ++w) {
-          const uint32_t hi = encode4(&y[k][4 * w], e);
+          // (within 448 all of them: no bounds; z - z makes the second code of NaN and infinities NaN)
+          const float f = pow2(-e), *v = &y[k][4 * w], z[4] = {v[0] * f, v[1] * f, v[2] * f, v[3] * f};
+          const uint32_t hi = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false), true);
           const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, 1.0f, true);
-          const float f = pow2(-e), back[4] = {a[0], a[1], b[0], b[1]};
+          const float back[4] = {a[0], a[1], b[0], b[1]};
           float rest[4];
 #pragma unroll
-          for (int m = 0; m < 4; ++m) rest[m] = 16.f * (y[k][4 * w + m] * f - back[m]);
+          for (int m = 0; m < 4; ++m) rest[m] = __builtin_fmaf(16.f, z[m] - back[m], z[m] - z[m]);
           qc[i][0][k][w] = (int)hi;
-          qc[i][1][k][w] = (int)encode4(rest, 0);
+          qc[i][1][k][w] = __builtin_amdgcn_cvt_pk_fp8_f32(rest[2], rest[3], __builtin_amdgcn_cvt_pk_fp8_f32(rest[0], rest[1], 0, false), true);
         }
     } else {
 #pragma unroll

@@ -194,6 +194,21 @@ def test_values_that_a_row_sees_pass(codes):
     assert bool(got[3:, 11].isinf().all()) and int((~got.isfinite()).sum()) == 6
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("draft", [1, 6, 20, 40])
+@pytest.mark.parametrize("codes", [True, False])
+def test_bad_queries_stay_in_their_rows(codes, draft, bad):
+    """A query with a non-finite element: its head of its token alone is NaN"""
+    c = Case(torch.bfloat16, codes, 128, 64, 4, 2, [(200, draft), (70, draft)], seed=15)
+    want = c.run()
+    row, head = draft + draft // 2, 3
+    c.q[row, head * 128 + 77] = bad
+    got = c.run()
+    keep = torch.ones_like(got, dtype=torch.bool)
+    keep[row, head * 64:(head + 1) * 64] = False
+    assert bool(got[~keep].isnan().all()) and torch.equal(got[keep], want[keep])
+
+
 @pytest.mark.parametrize("codes", [True, False])
 def test_pages_that_are_not_there(codes):
     """Page numbers outside the pools are not seen; lengths beyond the block table end with it"""
