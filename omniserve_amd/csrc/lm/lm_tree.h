@@ -32,6 +32,10 @@ constexpr int NO_WINDOW = INT32_MAX;
 // The newest position that a token does not see any more
 __device__ __forceinline__ int bound_of(const TreeArgs& p, int pos) { return p.window == NO_WINDOW ? INT32_MIN : max(pos, INT32_MIN + p.window) - p.window; }
 
+// A row's weights are relative to a maximum that is followed only when it has grown by so much (in powers of two): what has been added up is rescaled in a
+// few tiles, not in every second one
+constexpr float LAZY = 8.f;
+
 // Largest of the four lanes that share l15, by lane swaps (column_max goes through LDS: two latencies in every tile's chain)
 __device__ __forceinline__ float rows_max(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);

@@ -25,7 +25,7 @@ __device__ __forceinline__ float inverse_of(uint32_t w, int i) { return __uint_a
 template <int DK, int DV, int NR, bool CODES>
 struct Tree {
   static constexpr bool F16 = CODES && SPLIT;                     // weights of codes are one f16 operand
-  static constexpr float SHIFT = F16 ? 14.f : 0.f;
+  static constexpr float SHIFT = F16 ? 7.f : 0.f;                  // an f16 weight is at most 2^(LAZY + 7)
   static constexpr int CH = DK / 64, PF = 16 / FR, NKF = CH * PF, NVB = DV / 16;
   static constexpr int KT = CODES ? 64 : 32, NU = KT / 16;        // keys of a context tile
   static constexpr int STAGE = 64 * DV;                           // bytes of a wave's V tile: 64 rows of codes, 32 of bf16
@@ -58,9 +58,8 @@ struct Tree {
 #pragma unroll
       for (int r = 0; r < 4; ++r) t = fmaxf(t, x[u][r]);
     t = rows_max(t);
-    const float m_new = t <= NEG ? m_run[i] : fmaxf(m_run[i], t);
-    const float m_sub = (m_new <= NEG ? 0.f : m_new) - SHIFT;
-    const float alpha = __builtin_amdgcn_exp2f(m_run[i] - m_new);
+    const bool grows = t > m_run[i] + LAZY;      // (the first key's always; a NaN never)
+    const float m_new = grows ? t : m_run[i], m_sub = (m_new <= NEG ? 0.f : m_new) - SHIFT;
     float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -69,12 +68,14 @@ struct Tree {
         x[u][r] = __builtin_amdgcn_exp2f(x[u][r] - m_sub);
         sum = ONE ? sum + x[u][r] : __builtin_fmaf(x[u][r], inv[u][r], sum);
       }
-    l_run[i] = l_run[i] * alpha + (ONE ? sum * inv_all : sum);
-    m_run[i] = m_new;
-    if (__any(alpha != 1.0f)) {      // (the maximum settles after a few tiles)
+    if (__any(grows)) {
+      const float alpha = __builtin_amdgcn_exp2f(m_run[i] - m_new);
+      l_run[i] *= alpha;
 #pragma unroll
       for (int c = 0; c < NVB; ++c) acc[i][c] *= alpha;
     }
+    l_run[i] += ONE ? sum * inv_all : sum;
+    m_run[i] = m_new;
   }
 
   // What non-finite values among keys lo .. hi - 1 of a tile add to the rows that see them.  (They were left out of the products, where a weight of
@@ -397,7 +398,7 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
   int64_t part = 0;
   if (!piece_of<T::KT, 16 * NR>(p, s, part)) return;
   const int g = s.g, f0 = s.f0, drafted = s.drafted, gs = s.gs, R = s.R, r0 = s.rb * 16 * NR, length = s.length;
-  const int* bt = s.bt;
+  const __attribute__((address_space(4))) int* bt = (const __attribute__((address_space(4))) int*)(uintptr_t)s.bt;      // (scalar loads)
 
   T t(p);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);

@@ -24,10 +24,6 @@ __device__ __forceinline__ int key_swizzle(int row) {
   else return Tile<ROWB>::swizzle(row);
 }
 
-// A row's weights are relative to a maximum that is followed only when it has grown by so much (in powers of two): what has been added up is rescaled in a
-// few tiles, not in every second one
-constexpr float LAZY = 8.f;
-
 // Blocks of 16 rows of a wave: what 256 registers hold
 constexpr int row_blocks(int dk, int dv) { return dk > 128 || dv > 128 ? 1 : 2; }
 
