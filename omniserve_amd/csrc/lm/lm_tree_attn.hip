@@ -530,58 +530,61 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
   }
 }
 
-// Joins the pieces of a segment's rows: a wave a row, or (few rows, whose pieces are many) all four, a quarter of the pieces each.  Lane s holds the maximum
-// and sum of piece s of 64.
+// Joins the pieces of a segment's rows.  A lane has four columns, so that a wave has four, two or one rows (of 64, 128, 256), each with pieces of its own to
+// add up, or (few rows, whose pieces are many) the four waves of a workgroup the same rows and a quarter of the pieces each.  Lane l of a row holds the maximum
+// and sum of every l-th piece.
+template <int DV>
+constexpr int rows_of_wave() { return 256 / DV; }
 template <int ROWS, int DV>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p, int rows, int waves) {
-  __shared__ float res[3][DV + 1];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), each = 4 / waves, per = (rows + each - 1) / each;
-  const int seg = blockIdx.x / per, rr = (blockIdx.x - seg * per) * each + (waves == 1 ? wave : 0), w = waves == 1 ? 0 : wave;
+  constexpr int RW = rows_of_wave<DV>(), LR = 64 / RW;      // rows of a wave, lanes of a row
+  __shared__ f32x4 res[3][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane % LR, each = 4 / waves * RW, per = (rows + each - 1) / each;
+  const int seg = blockIdx.x / per, rr = (blockIdx.x - seg * per) * each + (waves == 1 ? wave * RW : 0) + lane / LR, w = waves == 1 ? 0 : wave;
   const int rb = seg % p.blocks, g = seg / p.blocks % p.G, b = seg / p.blocks / p.G, gs = p.H / p.G, r = rb * ROWS + rr;
-  const int f0 = min(max(p.first[b], 0), p.n), drafted = min(max(p.first[b + 1] - f0, 0), min(p.max_draft, p.n - f0)), parts = p.cuts[2 * seg + 1];
-  if (rr >= ROWS || r >= drafted * gs || parts == 1) return;      // (one piece: written by it)
-  const int64_t at0 = (int64_t)p.cuts[2 * seg] * ROWS + rr, step = (int64_t)((drafted * gs + ROWS - 1) / ROWS) * ROWS;
+  const int f0 = min(max(p.first[b], 0), p.n), drafted = min(max(p.first[b + 1] - f0, 0), min(p.max_draft, p.n - f0));
+  if (rb * ROWS >= drafted * gs) return;      // (such a segment is none, and nothing says how it is cut)
+  const int parts = p.cuts[2 * seg + 1];
+  if (parts == 1) return;                     // written by its piece
+  const bool mine = rr < ROWS && r < drafted * gs;
+  const int64_t at0 = (int64_t)p.cuts[2 * seg] * ROWS + min(rr, ROWS - 1), step = (int64_t)((drafted * gs + ROWS - 1) / ROWS) * ROWS;
   float m = NEG;
-  for (int s = lane; s < parts; s += 64) m = fmaxf(m, p.ml[2 * (at0 + s * step)]);
+  for (int s = l; s < parts; s += LR) m = fmaxf(m, p.ml[2 * (at0 + s * step)]);
 #pragma unroll
-  for (int k = 32; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
-  float sum = 0.f, y[DV / 64] = {};
-  for (int s0 = 0; s0 < parts; s0 += 64) {
-    float v[8][DV / 64];
+  for (int k = LR / 2; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
+  float sum = 0.f;
+  f32x4 y = zero4();
+  for (int s0 = 0; s0 < parts; s0 += LR) {
+    f32x4 v[8];
     auto load = [&](int s1) {
 #pragma unroll
-      for (int s = 0; s < 8; ++s)
-#pragma unroll
-        for (int c = 0; c < DV / 64; ++c) v[s][c] = s0 + s1 + s * waves < parts ? p.part[(at0 + (s0 + s1 + s * waves) * step) * DV + 64 * c + lane] : 0.f;
+      for (int s = 0; s < 8; ++s) v[s] = s0 + s1 + s * waves < parts ? *(const f32x4*)(p.part + (at0 + (s0 + s1 + s * waves) * step) * DV + 4 * l) : zero4();
     };
     load(w);      // (beside the sums' request)
-    const bool in = s0 + lane < parts;
-    const float ms = in ? p.ml[2 * (at0 + (s0 + lane) * step)] : NEG, ls = in ? p.ml[2 * (at0 + (s0 + lane) * step) + 1] : 0.f;
+    const bool in = s0 + l < parts;
+    const float ms = in ? p.ml[2 * (at0 + (s0 + l) * step)] : NEG, ls = in ? p.ml[2 * (at0 + (s0 + l) * step) + 1] : 0.f;
     const float f = ls != 0.f ? __builtin_amdgcn_exp2f(ms - m) : 0.f;
-    sum += wave_sum(f * ls);
-    for (int s1 = w; s1 < min(64, parts - s0); s1 += 8 * waves) {
+    float t = f * ls;
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const float u = s1 + s * waves < 64 ? __shfl(f, (s1 + s * waves) & 63, 64) : 0.f;
+    for (int k = LR / 2; k > 0; k >>= 1) t += __shfl_xor(t, k, 64);
+    sum += t;
+    const int end = min(LR, parts - s0);
+    for (int s1 = w; s1 < end; s1 += 8 * waves) {
 #pragma unroll
-        for (int c = 0; c < DV / 64; ++c) y[c] += u * v[s][c];
-      }
-      if (s1 + 8 * waves < min(64, parts - s0)) load(s1 + 8 * waves);
+      for (int s = 0; s < 8; ++s) y += (s1 + s * waves < LR ? __shfl(f, lane - l + (s1 + s * waves) % LR, 64) : 0.f) * v[s];
+      if (s1 + 8 * waves < end) load(s1 + 8 * waves);
     }
   }
   if (waves > 1) {      // (uniform over the workgroup, as are the returns above)
-    if (w > 0)
-#pragma unroll
-      for (int c = 0; c < DV / 64; ++c) res[w - 1][64 * c + lane] = y[c];
+    if (w > 0) res[w - 1][lane] = y;
     __syncthreads();
     if (w > 0) return;
-#pragma unroll
-    for (int c = 0; c < DV / 64; ++c) y[c] += res[0][64 * c + lane] + res[1][64 * c + lane] + res[2][64 * c + lane];
+    y += res[0][lane] + res[1][lane] + res[2][lane];
   }
-  const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+  if (!mine) return;
+  y *= sum != 0.f ? 1.0f / sum : 0.f;
   const int tk = f0 + r / gs, h = g * gs + r % gs;
-#pragma unroll
-  for (int c = 0; c < DV / 64; ++c) p.o[(int64_t)tk * p.ldo + (int64_t)h * DV + 64 * c + lane] = (elem_t)(y[c] * inv);
+  *(quad_t*)(p.o + (int64_t)tk * p.ldo + (int64_t)h * DV + 4 * l) = to_quad(y);
 }
 
 // Blocks of 16 rows of a workgroup
@@ -600,7 +603,7 @@ template <int ROWS>
 static void launch_merge(const TreeArgs& a, int dv, hipStream_t s) {
   const int rows = min(ROWS, a.max_draft * (a.H / a.G));      // of a segment, at most
   const int64_t segments = (int64_t)a.B * a.G * a.blocks;
-  const int waves = segments * rows <= 512 ? 4 : 1, each = 4 / waves;
+  const int waves = segments * rows <= 512 ? 4 : 1, each = 4 / waves * (256 / dv);
   const dim3 grid((unsigned)(segments * ((rows + each - 1) / each)));
   if (dv == 64) hipLaunchKernelGGL((tree_merge_kernel<ROWS, 64>), grid, dim3(256), 0, s, a, rows, waves);
   else if (dv == 128) hipLaunchKernelGGL((tree_merge_kernel<ROWS, 128>), grid, dim3(256), 0, s, a, rows, waves);
