@@ -35,6 +35,8 @@ __device__ __forceinline__ int bound_of(const TreeArgs& p, int pos) { return p.w
 // A row's weights are relative to a maximum that is followed only when it has grown by so much (in powers of two): what has been added up is rescaled in a
 // few tiles, not in every second one
 constexpr float LAZY = 8.f;
+// Values' exponents from which a weight times 2^-exponent is the probability: beside values of 2^40, what is lost is below 2^-30 of the largest
+constexpr int LOWEST = -63;
 
 // Largest of the four lanes that share l15, by lane swaps (column_max goes through LDS: two latencies in every tile's chain)
 __device__ __forceinline__ float rows_max(float v) {

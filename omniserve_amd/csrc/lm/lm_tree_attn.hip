@@ -15,7 +15,8 @@
 // w_j = 2^(s_j + e_j - m'), m' the running maximum of s_j + e_j, the outputs are sum w_j code_j and the sum of the probabilities is
 // sum w_j 2^(-e_j).  So w_j is at most 2^LAZY and is ONE f16 operand (11 bits, times 2^7 so that small ones stay normal) beside codes that f16
 // holds exactly; bf16 values need two bf16 operands for theirs (16 bits).  The drafted values, whose exponents nothing has taken out, are
-// divided by a power of two of their own.
+// divided by a power of two of their own.  A tile with rows of very small values, or none but zeros (2^-100), beside which the others' maximum leaves
+// such a weight nothing, multiplies its roots with 2^(-e) one by one: its rows count in the sum as all others do.
 #include "lm_tree.h"
 #include "omniserve_lm.h"
 
@@ -52,18 +53,27 @@ struct Tree {
     __builtin_amdgcn_wave_barrier();
   }
 
-  // x: scores times scale plus the values' exponents, unseen ones NEG; inv: 2^-exponent.  Leaves the weights in x.
+  // x: scores times scale plus the values' exponents, unseen ones NEG; inv: 2^-exponent; low: some exponent is below LOWEST.  Leaves the weights in x.
   template <int U, bool ONE>
-  __device__ __forceinline__ void softmax(int i, f32x4 (&x)[U], const f32x4 (&inv)[U], float inv_all) {
+  __device__ __forceinline__ void softmax(int i, f32x4 (&x)[U], const f32x4 (&inv)[U], float inv_all, bool low) {
     float t = NEG;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int r = 0; r < 4; ++r) t = fmaxf(t, x[u][r]);
     t = rows_max(t);
-    const bool grows = t > m_run[i] + LAZY;      // (the first key's always; a NaN never)
+    const bool grows = t > m_run[i] + (low ? 0.f : LAZY);      // (the first key's always; a NaN never)
     const float m_new = grows ? t : m_run[i], m_sub = (m_new <= NEG ? 0.f : m_new) - SHIFT;
-    float sum = 0.f;
+    float own = 0.f, sum = 0.f;
+    if (low) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float root = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][r], 0.5f, -0.5f * m_sub));
+          own = __builtin_fmaf(root * (ONE ? inv_all : inv[u][r]), root, own);
+        }
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -72,12 +82,12 @@ struct Tree {
         sum = ONE ? sum + x[u][r] : __builtin_fmaf(x[u][r], inv[u][r], sum);
       }
     if (__any(grows)) {
-      const float alpha = __builtin_amdgcn_exp2f(m_run[i] - m_new);
-      l_run[i] *= alpha;
+      const float root = __builtin_amdgcn_exp2f(0.5f * (m_run[i] - m_new)), alpha = root * root;
+      l_run[i] = l_run[i] * root * root;      // (alpha may be too small where the sum, of 2^100 for values of zero, is not)
 #pragma unroll
       for (int c = 0; c < NVB; ++c) acc[i][c] *= alpha;
     }
-    l_run[i] += ONE ? sum * inv_all : sum;
+    l_run[i] += low ? own : ONE ? sum * inv_all : sum;
     m_run[i] = m_new;
   }
 
@@ -173,6 +183,10 @@ struct Tree {
     for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int r = 0; r < 4; ++r) { ev[u][r] = exponent_of(c.vx[u], r); inv[u][r] = inverse_of(c.vx[u], r); }
+    uint32_t high = ~0u;      // a byte's highest bit: it is 64 at least
+#pragma unroll
+    for (int u = 0; u < NU; ++u) high &= c.vx[u] | c.vx[u] << 1;
+    const bool low_values = __any(~high & 0x80808080u);
     if constexpr (SPLIT) {
       if (edge) {
         const int first = here(lane / (DV / 16));
@@ -213,7 +227,7 @@ struct Tree {
             x[i][u][r] = (int)(key >= lo) & (int)(key < hi) & (int)(kb + key > low[i]) ? x[i][u][r] : NEG;
           }
       }
-      softmax<NU, false>(i, x[i], inv, 1.f);
+      softmax<NU, false>(i, x[i], inv, 1.f, low_values);
       if constexpr (SPLIT) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) pq[i][u] = (f16x4){(_Float16)x[i][u][0], (_Float16)x[i][u][1], (_Float16)x[i][u][2], (_Float16)x[i][u][3]};
@@ -355,7 +369,7 @@ struct Tree {
 #pragma unroll
           for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, key + 16 * u + r) ? x[i][u][r] : NEG;
       }
-      softmax<2, true>(i, x[i], x[i], pow2(-e));
+      softmax<2, true>(i, x[i], x[i], pow2(-e), e < LOWEST);
 #pragma unroll
       for (int u = 0; u < 2; ++u) split_quad(x[i][u], pq[i][u]);
     }
@@ -517,9 +531,9 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
       float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const float f = wl[w][rr] != 0.f ? __builtin_amdgcn_exp2f(wm[w][rr] - m) : 0.f;
-        sum += f * wl[w][rr];
-        y += f * *(const f32x4*)&res[w][rr][d];
+        const float root = wl[w][rr] != 0.f ? __builtin_amdgcn_exp2f(0.5f * (wm[w][rr] - m)) : 0.f;
+        sum += wl[w][rr] * root * root;
+        y += root * root * *(const f32x4*)&res[w][rr][d];
       }
       if (!s.whole) {
         const int64_t at = part + 16 * i + rr;
@@ -566,8 +580,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p, int rows, i
     load(w);      // (beside the sums' request)
     const bool in = s0 + l < parts;
     const float ms = in ? p.ml[2 * (at0 + (s0 + l) * step)] : NEG, ls = in ? p.ml[2 * (at0 + (s0 + l) * step) + 1] : 0.f;
-    const float f = ls != 0.f ? __builtin_amdgcn_exp2f(ms - m) : 0.f;
-    float t = f * ls;
+    const float root = ls != 0.f ? __builtin_amdgcn_exp2f(0.5f * (ms - m)) : 0.f, f = root * root;
+    float t = ls * root * root;
 #pragma unroll
     for (int k = LR / 2; k > 0; k >>= 1) t += __shfl_xor(t, k, 64);
     sum += t;

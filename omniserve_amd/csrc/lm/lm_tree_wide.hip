@@ -184,8 +184,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   }
   const float inv_scale = 1.0f / p.scale;
 
-  // x: scores (with e / scale), unseen ones NEG -> weights
-  auto softmax = [&](int i, auto& x, const auto& inv, auto one, float inv_all) {
+  // x: scores (with e / scale), unseen ones NEG -> weights; low: some exponent is below LOWEST
+  auto softmax = [&](int i, auto& x, const auto& inv, auto one, float inv_all, bool low) {
     constexpr int U = sizeof(x) / sizeof(f32x4);
     float t = NEG;
 #pragma unroll
@@ -194,9 +194,18 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       for (int r = 0; r < 4; ++r) t = fmaxf(t, x[u][r]);
     t = rows_max(t);
     t = t <= NEG ? NEG : t * p.scale;
-    const bool grows = t > m_run[i] + LAZY;      // (the first key's always; a NaN never)
+    const bool grows = t > m_run[i] + (low ? 0.f : LAZY);      // (the first key's always; a NaN never)
     const float m_new = grows ? t : m_run[i], m_sub = (m_new <= NEG ? 0.f : m_new) - W::SHIFT;
-    float sum = 0.f;
+    float own = 0.f, sum = 0.f;
+    if (low) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float root = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][r], 0.5f * p.scale, -0.5f * m_sub));
+          own = __builtin_fmaf(root * (one.value ? inv_all : inv[u][r]), root, own);
+        }
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -206,12 +215,12 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
         else sum = __builtin_fmaf(x[u][r], inv[u][r], sum);
       }
     if (__any(grows)) {
-      const float alpha = __builtin_amdgcn_exp2f(m_run[i] - m_new);
-      l_run[i] *= alpha;
+      const float root = __builtin_amdgcn_exp2f(0.5f * (m_run[i] - m_new)), alpha = root * root;
+      l_run[i] = l_run[i] * root * root;      // (alpha may be too small where the sum, of 2^100 for values of zero, is not)
 #pragma unroll
       for (int c = 0; c < NVB; ++c) acc[i][c] *= alpha;
     }
-    l_run[i] += one.value ? sum * inv_all : sum;
+    l_run[i] += low ? own : one.value ? sum * inv_all : sum;
     m_run[i] = m_new;
   };
   auto wave_sync = [&]() {
@@ -254,7 +263,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, key + 16 * u + r) ? x[i][u][r] : NEG;
       }
-      softmax(i, x[i], x[i], Yes(), pow2(-e));
+      softmax(i, x[i], x[i], Yes(), pow2(-e), e < LOWEST);
 #pragma unroll
       for (int u = 0; u < 2; ++u) split_quad(x[i][u], pq[i][u]);
     }
@@ -338,8 +347,10 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       }
       if (live) {
         f32x4* mine = (f32x4*)own;      // e / scale of 64 keys, then 2^-e
+        bool low_values;
         {
           const uint32_t b = exps[64 + lane];
+          low_values = __any((int)b < LOWEST + 127);
           wave_sync();
           ((float*)own)[lane] = ((float)b - 127.f) * inv_scale;
           ((float*)own)[64 + lane] = __uint_as_float((254 - b) << 23);
@@ -389,7 +400,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
               for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, key + 16 * u + r) ? x[i][u][r] : NEG;
           }
-          softmax(i, x[i], inv, No(), 1.f);
+          softmax(i, x[i], inv, No(), 1.f, low_values);
 #pragma unroll
           for (int u = 0; u < NU; ++u) pq[i][u] = (f16x4){(_Float16)x[i][u][0], (_Float16)x[i][u][1], (_Float16)x[i][u][2], (_Float16)x[i][u][3]};
         }

@@ -376,3 +376,43 @@ def test_a_chain_is_its_tokens_in_turn():
         ref = torch.empty(1, H * d, dtype=dtype, device=dev())
         ops.attn_decode(row, None, 0.0, none, torch.tensor([at], dtype=torch.int32, device=dev()), slot, kc, vc, c.bt, None, ref, None, 1, c.scale, NO_WINDOW, H, G, d, d)
         assert ((ref[0].double() - got[i].double()).abs().view(H, d) <= 2 * bound[i]).all()
+
+
+@pytest.mark.parametrize("first", ["zeros", "loud"])
+@pytest.mark.parametrize("loud", [2.0 ** 20, 2.0 ** 40, 2.0 ** 80])
+@pytest.mark.parametrize("draft", [1, 26, 64])
+def test_zeros_beside_loud_values(draft, loud, first):
+    """Rows of zeros have the lowest exponent; they take their part of the sum whatever the others' is, in a tile of their own or not, in one piece or several"""
+    for context in (300, 3000):
+        c = Case(torch.bfloat16, True, 128, 128, 4, 2, [(context, draft), (context, draft)], seed=draft)
+        c.cache[3].add_(int(math.log2(loud)))
+        zeros = torch.zeros(context, dtype=torch.bool, device=dev())
+        zeros[:context // 2] = True
+        zeros = zeros if first == "zeros" else ~zeros
+        zeros[::3] = True
+        for b in range(2):
+            for page in range(-(-context // PAGE)):
+                at = zeros[page * PAGE:(page + 1) * PAGE].nonzero()[:, 0]
+                for t, x in zip((c.cache[1], c.cache[3]), (0, 27)):
+                    t[int(c.bt[b, page]), :, at] = x
+        c.check(c.run())
+
+
+@pytest.mark.parametrize("draft", [1, 26, 64])
+def test_nothing_but_zeros(draft):
+    """Many keys of the lowest exponent, whose scores rise: the sum stays finite"""
+    c = Case(torch.bfloat16, True, 128, 128, 4, 2, [(40000, draft)], seed=draft)
+    c.cache[1].zero_()
+    c.cache[3].fill_(27)
+    c.check(c.run())
+    c.v *= 2.0 ** 60
+    c.check(c.run())
+
+
+def test_more_sequences_than_a_wave_has_lanes():
+    """Segments are dealt out by one wave: 64 sequences, one more and many, some without tokens"""
+    for n in (64, 65, 150):
+        for draft in (1, 12, 40):
+            c = Case(torch.bfloat16, True, 64, 64, 4, 2, [((i * 37) % 700, draft if i % 5 else 0) for i in range(n)], seed=n)
+            c.check(c.run())
+            c.check(c.run(max_context=5000))
