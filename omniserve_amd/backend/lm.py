@@ -225,7 +225,7 @@ class LmOps:
         bt[b].  A token sees the cached keys and, of its sequence, the drafted ones whose bit is set in mask [tokens, words] (int64, tree_masks); with a
         window only those at positions above its pos - window.  Rows that see nothing are zero; rows of no sequence stay as they are.  cache: KvCodes, or
         (keys, values) [pages, kv heads, 64, size] of elements.  max_context: a bound of the lengths, by which the work is divided (longer ones are
-        attended to as well)."""
+        attended to as well).  scale: 2^-60 to 2^60."""
         return self._x.tree_attn(q, k, v, mask, first, pos, cache, bt, length, scale, window, max_draft, max_context, out)
 
     def linear_prefill(self, x, o, state, seg_state, seg, seg_len, multi, log2_decay, heads, dk, dv, act):

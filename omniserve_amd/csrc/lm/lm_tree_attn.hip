@@ -656,6 +656,9 @@ static Plan plan_of(int B, int max_draft, int max_context, int H, int G, int dk,
 
 using namespace lm;
 
+// (an exponent of 127 over the scale is far above NEG, and a score times the scale finite)
+static constexpr float MIN_SCALE = 0x1p-60f;
+
 extern "C" int64_t lm_tree_attn_scratch(int B, int max_draft, int max_context, int H, int G, int dk, int dv, int codes) {
   if (B <= 0 || G <= 0 || H <= 0 || H % G || max_draft <= 0 || max_context < 0 || (int64_t)max_draft * H > 1 << 24) return 0;
   return plan_of(B, max_draft, max_context, H, G, dk, dv, codes != 0).scratch;
@@ -665,7 +668,7 @@ extern "C" int lm_tree_attn(const void* q, int64_t ldq, const void* k, int64_t l
                             const uint8_t* ve, int64_t pages, const int* bt, int bt_stride, int bt_width, const int* length, const int* first, const int* pos,
                             const int64_t* mask, int words, void* o, int64_t ldo, float* part, float scale, int window, int B, int n, int max_draft,
                             int max_context, int H, int G, int dk, int dv, void* stream) {
-  if (B < 0 || n < 0 || max_draft < 0 || G <= 0 || H <= 0 || H % G || !(scale > 0.f) || window <= 0 || words < 0 || bt_width < 0 || bt_stride < bt_width ||
+  if (B < 0 || n < 0 || max_draft < 0 || G <= 0 || H <= 0 || H % G || !(scale >= MIN_SCALE && scale <= 1.0f / MIN_SCALE) || window <= 0 || words < 0 || bt_width < 0 || bt_stride < bt_width ||
       bt_width > INT32_MAX / PAGE || pages < 0 || pages > INT32_MAX / PAGE || (bt_width > 0 && pages == 0) || max_context < 0 || (ke == nullptr) != (ve == nullptr) || ldq % FR || ldk % FR || ldv % FR || ldo % 4 || (int64_t)max_draft * H > 1 << 24 ||
       // (tiles are counted in 32 bits)
       (int64_t)B * G * (max_draft * (H / G) / 16 + 1) * (2 * (int64_t)bt_width + max_draft / 32 + 2) > INT32_MAX)

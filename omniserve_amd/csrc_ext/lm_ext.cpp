@@ -186,7 +186,7 @@ class Ops {
     index(length, B, "length");
     need(bt.scalar_type() == torch::kInt32 && bt.dim() == 2 && bt.size(0) == B && (bt.stride(1) == 1 || bt.size(1) <= 1), "bt: int32 [sequences, pages]");
     need(bt.size(1) == 0 || s.pages > 0, "a block table needs pages");
-    need(scale > 0 && (!window || *window > 0), "scale and window are positive");
+    need(scale >= 0x1p-60 && scale <= 0x1p60 && (!window || *window > 0), "scale: 2^-60 to 2^60; window: positive");
     need(max_context >= 0, "max_context is a number of keys");
     if (out) {
       rows(*out, H * s.dv, n, "out");

@@ -148,6 +148,10 @@ def test_tree_attention_refuses(ops):
     bad("bt", bt=torch.zeros(4, 2, dtype=I32).t())
     bad("scale", scale=0.0)
     bad("scale", scale=float("nan"))
+    for scale in (-0.1, float("inf"), 1e300, 2.0 ** 61, 2.0 ** -61, 1e-300):
+        bad("scale", scale=scale)
+    bad("GPU", scale=2.0 ** -60)
+    bad("GPU", scale=2.0 ** 60)
     bad("window", window=0)
     bad("window", window=-3)
     bad("max_context", max_context=-1)
@@ -175,7 +179,7 @@ def test_library_refuses(ops):
     tree = lambda B=1, n=1, draft=1, H=2, G=1, dk=64, dv=64, width=2, pages=3, context=100, scale=f, window=1, ldq=128, ke=64, ve=64, q=64: h.lm_tree_attn(      # noqa: E731
         q, ldq, 64, 64, 64, 64, 64, 64, ke, ve, pages, 64, width, width, 64, 64, 64, 64, 1, 64, 128, None, scale, window, B, n, draft, context, H, G, dk, dv, None)
     assert tree(B=0) == tree(n=0) == tree(draft=0) == 0
-    for bad in (dict(H=3, G=2), dict(dk=80), dict(dv=192), dict(pages=0), dict(context=-1), dict(width=1 << 26, pages=1 << 20), dict(scale=0.0), dict(scale=float("nan")), dict(window=0),
+    for bad in (dict(H=3, G=2), dict(dk=80), dict(dv=192), dict(pages=0), dict(context=-1), dict(width=1 << 26, pages=1 << 20), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=2.0 ** -61), dict(scale=2.0 ** 61), dict(window=0),
                 dict(ldq=129), dict(ke=None), dict(ve=None), dict(q=None), dict(q=72), dict(B=-1)):
         assert tree(**bad) == -22, bad
 

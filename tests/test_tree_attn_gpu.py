@@ -416,3 +416,12 @@ def test_more_sequences_than_a_wave_has_lanes():
             c = Case(torch.bfloat16, True, 64, 64, 4, 2, [((i * 37) % 700, draft if i % 5 else 0) for i in range(n)], seed=n)
             c.check(c.run())
             c.check(c.run(max_context=5000))
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -60, 2.0 ** -12, 1.0])
+@pytest.mark.parametrize("draft", [1, 64])
+@pytest.mark.parametrize("codes", [True, False])
+def test_scales(codes, draft, scale):
+    c = Case(torch.bfloat16, codes, 128, 128, 4, 2, [(500, draft), (70, draft)], seed=draft)
+    c.scale = scale
+    c.check(c.run())
