@@ -221,9 +221,9 @@ class LmOps:
 
     def tree_attn(self, q, k, v, mask, first, pos, cache, bt, length, scale, *, window=None, max_draft, max_context, out=None):
         """Attention of drafted tokens (rows q [heads * dk], k, v [kv heads * size], turned already) over a paged cache -> [tokens, heads * dv].
-        Sequence b has the tokens first[b] .. first[b + 1] - 1, at most max_draft (further ones are left out), and length[b] cached keys in the pages
-        bt[b].  A token sees the cached keys and, of its sequence, the drafted ones whose bit is set in mask [tokens, words] (int64, tree_masks); with a
-        window only those at positions above its pos - window.  Rows that see nothing are zero; rows of no sequence stay as they are.  cache: KvCodes, or
+        Sequence b has the tokens first[b] .. first[b + 1] - 1 (first does not descend), at most max_draft (further ones are left out), and length[b] cached
+        keys in the pages bt[b].  A token sees the cached keys and, of its sequence, the drafted ones whose bit is set in mask [tokens, words] (int64, tree_masks); with a
+        window only those at positions above its pos - window.  Rows that see nothing are zero; rows of no sequence stay as they are (without out they are unspecified).  cache: KvCodes, or
         (keys, values) [pages, kv heads, 64, size] of elements.  max_context: a bound of the lengths, by which the work is divided (longer ones are
         attended to as well).  scale: 2^-60 to 2^60."""
         return self._x.tree_attn(q, k, v, mask, first, pos, cache, bt, length, scale, window, max_draft, max_context, out)
