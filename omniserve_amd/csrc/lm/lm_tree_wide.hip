@@ -8,7 +8,7 @@
 //     twice the rate of bf16: as long as one, and no conversion;
 //   a value's exponent (lm_tree_attn.hip) is the products' initial accumulator, e / scale;
 //   2^-e and e / scale are formed by one lane per key and read back from LDS.
-// 4 trees of 64 over 32768 keys, 32 heads over 8: 172 us, 0.80 PFLOP/s; matrix units busy 37 % of the time, vector units 56, no LDS conflicts
+// 4 trees of 64 over 32768 keys, 32 heads over 8: 174 us, 0.77 PFLOP/s; matrix units busy 36 % of the time, vector units 56, no LDS conflicts
 // (workgroups of half the rows 188 for 183 us; staggered starts 173 for 176; the products at higher priority: no change).
 #include "lm_tree.h"
 
