@@ -205,7 +205,7 @@ class LmOps:
 
     def rope(self, x, freq, pos, heads, dk, *, pairing="neighbours", factor=1.0, out=None):
         """The first 2 * len(freq) dimensions of `heads` heads of dk turned by pos * freq (float64), the cosine and sine times factor -> out:
-        x itself (in place), memory that does not overlap x, or (None) new rows [tokens, heads * dk].  Rows of a negative position are left out."""
+        x itself (in place), memory that does not overlap x, or (None) new rows [tokens, heads * dk].  Rows of a negative position are left out (new ones are unspecified)."""
         return self._x.rope(x, freq, pos, heads, dk, pairing, factor, out)
 
     def kv_store(self, x, cache, slot, heads, *, freq=None, pos=None, pairing="neighbours", factor=1.0, q_out=None, rows=None):
@@ -225,7 +225,7 @@ class LmOps:
         keys in the pages bt[b].  A token sees the cached keys and, of its sequence, the drafted ones whose bit is set in mask [tokens, words] (int64, tree_masks); with a
         window only those at positions above its pos - window.  Rows that see nothing are zero; rows of no sequence stay as they are (without out they are unspecified).  cache: KvCodes, or
         (keys, values) [pages, kv heads, 64, size] of elements.  max_context: a bound of the lengths, by which the work is divided (longer ones are
-        attended to as well).  scale: 2^-60 to 2^60."""
+        attended to as well).  scale: 2^-60 to 2^60.  out: memory of its own."""
         return self._x.tree_attn(q, k, v, mask, first, pos, cache, bt, length, scale, window, max_draft, max_context, out)
 
     def linear_prefill(self, x, o, state, seg_state, seg, seg_len, multi, log2_decay, heads, dk, dv, act):

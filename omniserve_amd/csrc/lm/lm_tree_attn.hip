@@ -675,7 +675,7 @@ extern "C" int lm_tree_attn(const void* q, int64_t ldq, const void* k, int64_t l
     return LM_EINVAL;
   if (B == 0 || n == 0 || max_draft == 0) return LM_OK;
   if (!q || !k || !v || !length || !first || !pos || !mask || !o || (bt_width > 0 && (!bt || !kc || !vc)) ||
-      ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)part) % 16 || (uintptr_t)o % 8 || (uintptr_t)ve % 4)
+      ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)ke | (uintptr_t)ve | (uintptr_t)part) % 16 || (uintptr_t)o % 8)
     return LM_EINVAL;
   TreeArgs a{};
   a.q = (const elem_t*)q; a.ldq = ldq; a.k = (const elem_t*)k; a.ldk = ldk; a.v = (const elem_t*)v; a.ldv = ldv;

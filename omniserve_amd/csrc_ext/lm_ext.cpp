@@ -169,6 +169,7 @@ class Ops {
               const std::optional<int64_t>& window, int64_t max_draft, int64_t max_context, const OptT& out) const {
     const bool codes = cache.size() == 4;
     const Sizes s = pools(cache, codes);
+    for (const T& t : cache) need((uintptr_t)t.data_ptr() % 16 == 0, "cache: pools at 16 bytes");
     need(q.dim() == 2 && s.G > 0, "q: rows, over kv heads");
     need(length.dim() == 1, "length: a vector");
     const int64_t n = q.size(0), B = length.size(0), H = q.size(1) / s.dk;

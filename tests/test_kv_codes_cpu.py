@@ -131,6 +131,9 @@ def test_tree_attention_refuses(ops):
     bad("GPU", window=7, max_draft=64)
     bad("pools", cache=tuple(p.to(torch.float16) for p in plain))
     bad("cache", cache=cache[:3])
+    for i in range(4):      # (a view that begins between two 16-byte boundaries)
+        odd = torch.zeros(cache[i].numel() + 4, dtype=torch.uint8)[4:].view(cache[i].shape)
+        bad("16 bytes", cache=(*cache[:i], odd, *cache[i + 1:]))
     bad("q:", q=torch.zeros(n, 3 * 64, dtype=t))
     bad("q:", q=torch.zeros(n, 4 * 64 + 1, dtype=t))
     bad("q:", q=ok["q"].to(torch.float16))
@@ -180,7 +183,7 @@ def test_library_refuses(ops):
         q, ldq, 64, 64, 64, 64, 64, 64, ke, ve, pages, 64, width, width, 64, 64, 64, 64, 1, 64, 128, None, scale, window, B, n, draft, context, H, G, dk, dv, None)
     assert tree(B=0) == tree(n=0) == tree(draft=0) == 0
     for bad in (dict(H=3, G=2), dict(dk=80), dict(dv=192), dict(pages=0), dict(context=-1), dict(width=1 << 26, pages=1 << 20), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=2.0 ** -61), dict(scale=2.0 ** 61), dict(window=0),
-                dict(ldq=129), dict(ke=None), dict(ve=None), dict(q=None), dict(q=72), dict(B=-1)):
+                dict(ldq=129), dict(ke=72), dict(ve=72), dict(ve=68), dict(ke=None), dict(ve=None), dict(q=None), dict(q=72), dict(B=-1)):
         assert tree(**bad) == -22, bad
 
 
