@@ -56,7 +56,9 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   if (!piece_of<KT, W::ROWS>(p, s, part)) return;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l15 = lane & 15, l4 = lane >> 4;
   uint8_t* own = lds + W::NBUF * W::SLOT + wave * W::OWN;
-  int* shared = (int*)(lds + W::NBUF * W::SLOT + NW * W::OWN);      // smallest, largest of the rows' bounds; a tile's largest value, whether it has non-finite ones
+  // smallest, largest of the rows' bounds; whether a context tile has non-finite values; a drafted tile, its largest value (words of their own: a wave may
+  // still have to read the last context tile's when another one clears them)
+  int* shared = (int*)(lds + W::NBUF * W::SLOT + NW * W::OWN);
   const int r0 = s.rb * W::ROWS + wave * 16 * NR;
   const bool live = r0 < s.R;                                         // (a wave without rows fetches its pieces and waits with the others)
 
@@ -440,7 +442,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       uint8_t* vt = lds + E::KBYTES;
       // Values pass through registers: non-finite ones are left out, codes' kernels divide by a power of two
       constexpr int VF = (32 * DV / 8 + 64 * NW - 1) / (64 * NW);
-      if (tid == 0) { shared[2] = 0; shared[3] = 0; }
+      if (tid == 0) { shared[3] = 0; shared[4] = 0; }
       frag_t vf[VF];
       bool bad = false;
       float top = 0.f;
@@ -467,12 +469,12 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       if constexpr (CODES) {
 #pragma unroll
         for (int m = 32; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-        if (lane == 0) atomicMax(&shared[3], (int)__float_as_uint(top));      // (not negative: ordered like whole numbers)
+        if (lane == 0) atomicMax(&shared[4], (int)__float_as_uint(top));      // (not negative: ordered like whole numbers)
       }
-      if (__any(bad) && lane == 0) atomicOr(&shared[2], 1);
+      if (__any(bad) && lane == 0) atomicOr(&shared[3], 1);
       __syncthreads();
-      bad = shared[2] != 0;
-      const int e = CODES ? row_exponent(__uint_as_float((uint32_t)shared[3])) : 0;
+      bad = shared[3] != 0;
+      const int e = CODES ? row_exponent(__uint_as_float((uint32_t)shared[4])) : 0;
       const float f = pow2(-e);
 #pragma unroll
       for (int k = 0; k < VF; ++k) {

@@ -1,0 +1,67 @@
+"""Attention of drafted tokens where it can go wrong: values that are not finite in every kind of tile, exponents and magnitudes far apart, segments cut
+into many pieces, few and many rows alike.  Against 64 bits; infinities and NaN are told apart."""
+import math
+
+import pytest
+import torch
+
+from tests.kv_codes_util import PAGE, attention, attention_bound
+from tests.test_tree_attn_gpu import NO_WINDOW, Case
+from tests.util import dev
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+DRAFTS = [1, 12, 20, 64, 150]      # rows of 2 heads per kv head: one block of 16, two, and the kernel of many rows with 2, 4 and 8 waves
+
+
+def _limits(c, window):
+    """[tokens, heads, dv]: 0 where every value that a row sees is finite, else what their sum is, whatever the weights: inf, -inf or nan"""
+    n, (kpool, vpool) = c.q.shape[0], c.pools()
+    out = torch.zeros(n, c.H, c.dv, dtype=torch.float64, device=dev())
+    first = c.first.tolist()
+    for b, ln in enumerate(c.length.tolist()):
+        f0, t = first[b], min(first[b + 1] - first[b], c.max_draft)
+        if t <= 0:
+            continue
+        pages = c.bt[b, :-(-ln // PAGE)].long()
+        v = torch.cat((vpool[pages].transpose(1, 2).reshape(-1, c.G, c.dv)[:ln], c.v[f0:f0 + t].double().view(t, c.G, c.dv)))
+        p, j = c.pos[f0:f0 + t].long(), torch.arange(t, device=dev())
+        bits = (c.mask[f0:f0 + t][:, j // 64] >> (j % 64)) & 1
+        where = torch.cat((torch.arange(ln, device=dev()), p))
+        seen = torch.cat((torch.ones(t, ln, dtype=torch.bool, device=dev()), bits.bool()), 1) & (where[None] > p[:, None] - window)
+        for key in (~v.isfinite()).flatten(1).any(1).nonzero()[:, 0].tolist():
+            bad = torch.where(v[key].isfinite(), 0.0, v[key]).repeat_interleave(c.H // c.G, 0)
+            out[f0:f0 + t] += torch.where(seen[:, key, None, None], bad[None], 0.0)
+    return out
+
+
+def _check(c, got, window=None):
+    """Where nothing but finite values is seen: within the bound of the finite ones; elsewhere the right kind of infinity, or NaN"""
+    n, window = c.q.shape[0], window or NO_WINDOW
+    want = _limits(c, window)
+    assert not bool((c.first[1:] - c.first[:-1] > c.max_draft).any())
+    ref = attention(c.q.double().view(n, c.H, c.dk), c.k.double().view(n, c.G, c.dk), c.v.double().view(n, c.G, c.dv).nan_to_num(0, 0, 0), c.mask, c.first.cpu(), c.pos,
+                    *(t.nan_to_num(0, 0, 0) for t in c.pools()), c.bt, c.length, c.scale, window, c.max_draft, c.H // c.G)
+    got = got.double().view(n, c.H, c.dv)
+    sick = want != 0      # (NaN is not 0)
+    assert torch.equal(got[sick].isnan(), want[sick].isnan()) and torch.equal(got[sick].nan_to_num(0), want[sick].nan_to_num(0))
+    over = ((got - ref[0]).abs() / attention_bound(c.dtype, c.codes, c.dk, *ref))[~sick]
+    assert over.numel() == 0 or float(over.max()) <= 1.0, float(over.max())
+
+
+def _spoil(c, b, key, bad, col=5):
+    """a cached value of sequence b"""
+    page, at = int(c.bt[b, key // PAGE]), key % PAGE
+    c.cache[1][page, 0, at, col] = 0x7f if c.codes else bad
+
+
+@pytest.mark.parametrize("draft", DRAFTS)
+@pytest.mark.parametrize("codes", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_bad_value_of_the_last_page_reaches_every_row(dtype, codes, draft):
+    """The last context tile, partly filled, holds it; drafted tiles follow"""
+    for n in (70, 300, 1001):
+        c = Case(dtype, codes, 128, 64, 4, 2, [(n, draft), (n // 2, draft)], seed=draft + n)
+        _spoil(c, 0, n - 1, -math.inf)
+        _spoil(c, 1, n // 2 - 1, math.inf, 63)
+        _check(c, c.run())
