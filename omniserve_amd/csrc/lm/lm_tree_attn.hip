@@ -575,7 +575,10 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p, int rows, i
     f32x4 v[8];
     auto load = [&](int s1) {
 #pragma unroll
-      for (int s = 0; s < 8; ++s) v[s] = s0 + s1 + s * waves < parts ? *(const f32x4*)(p.part + (at0 + (s0 + s1 + s * waves) * step) * DV + 4 * l) : zero4();
+      for (int s = 0; s < 8; ++s) {      // (of this round's: the next one's would be read twice, and zero times an infinity is NaN)
+        const int at = s1 + s * waves;
+        v[s] = at < min(LR, parts - s0) ? *(const f32x4*)(p.part + (at0 + (s0 + at) * step) * DV + 4 * l) : zero4();
+      }
     };
     load(w);      // (beside the sums' request)
     const bool in = s0 + l < parts;

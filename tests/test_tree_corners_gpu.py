@@ -65,3 +65,15 @@ def test_a_bad_value_of_the_last_page_reaches_every_row(dtype, codes, draft):
         _spoil(c, 0, n - 1, -math.inf)
         _spoil(c, 1, n // 2 - 1, math.inf, 63)
         _check(c, c.run())
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (64, 256)])
+@pytest.mark.parametrize("heads", [2, 64])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_bad_value_in_any_of_many_pieces(dtype, bad, heads, dk, dv):
+    """One token whose keys are cut into more pieces than a row has lanes when they are joined; the value lies in the partly filled last page, behind all others"""
+    c = Case(dtype, False, dk, dv, heads, 2, [(9001, 1)], seed=dk + heads)
+    c.scale = 2.0 ** -9      # (weights of one size)
+    _spoil(c, 0, 9000, bad)
+    _check(c, c.run())
