@@ -38,6 +38,11 @@ constexpr float LAZY = 8.f;
 // Values' exponents from which a weight times 2^-exponent is the probability: beside values of 2^40, what is lost is below 2^-30 of the largest
 constexpr int LOWEST = -63;
 
+// f * y for sums that are brought to a larger maximum.  An infinite value that a row sees counts whatever its weight is, so where the factor is zero in 32 bits
+// it stays what it is.
+__device__ __forceinline__ float rescaled(float f, float y) { return fabsf(y) < __builtin_inff() ? f * y : y; }
+__device__ __forceinline__ f32x4 rescaled(float f, f32x4 y) { return (f32x4){rescaled(f, y[0]), rescaled(f, y[1]), rescaled(f, y[2]), rescaled(f, y[3])}; }
+
 // Largest of the four lanes that share l15, by lane swaps (column_max goes through LDS: two latencies in every tile's chain)
 __device__ __forceinline__ float rows_max(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);

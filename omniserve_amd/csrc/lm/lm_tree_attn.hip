@@ -85,7 +85,7 @@ struct Tree {
       const float root = __builtin_amdgcn_exp2f(0.5f * (m_run[i] - m_new)), alpha = root * root;
       l_run[i] = l_run[i] * root * root;      // (alpha may be too small where the sum, of 2^100 for values of zero, is not)
 #pragma unroll
-      for (int c = 0; c < NVB; ++c) acc[i][c] *= alpha;
+      for (int c = 0; c < NVB; ++c) acc[i][c] = rescaled(alpha, acc[i][c]);
     }
     l_run[i] += low ? own : ONE ? sum * inv_all : sum;
     m_run[i] = m_new;
@@ -533,7 +533,7 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
       for (int w = 0; w < NW; ++w) {
         const float root = wl[w][rr] != 0.f ? __builtin_amdgcn_exp2f(0.5f * (wm[w][rr] - m)) : 0.f;
         sum += wl[w][rr] * root * root;
-        y += root * root * *(const f32x4*)&res[w][rr][d];
+        y += rescaled(root * root, *(const f32x4*)&res[w][rr][d]);
       }
       if (!s.whole) {
         const int64_t at = part + 16 * i + rr;
@@ -591,7 +591,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p, int rows, i
     const int end = min(LR, parts - s0);
     for (int s1 = w; s1 < end; s1 += 8 * waves) {
 #pragma unroll
-      for (int s = 0; s < 8; ++s) y += (s1 + s * waves < LR ? __shfl(f, lane - l + (s1 + s * waves) % LR, 64) : 0.f) * v[s];
+      for (int s = 0; s < 8; ++s) y += rescaled(s1 + s * waves < LR ? __shfl(f, lane - l + (s1 + s * waves) % LR, 64) : 0.f, v[s]);
       if (s1 + 8 * waves < end) load(s1 + 8 * waves);
     }
   }

@@ -77,3 +77,18 @@ def test_a_bad_value_in_any_of_many_pieces(dtype, bad, heads, dk, dv):
     c.scale = 2.0 ** -9      # (weights of one size)
     _spoil(c, 0, 9000, bad)
     _check(c, c.run())
+
+
+@pytest.mark.parametrize("draft", DRAFTS)
+@pytest.mark.parametrize("context", [70, 3000])
+@pytest.mark.parametrize("codes", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_an_infinite_value_of_no_weight(dtype, codes, context, draft):
+    """Scores so far apart that the weight of the infinite value, and the factor of the piece that holds it, are zero in 32 bits: it counts all the same"""
+    for scale in (8.0, 30.0):
+        c = Case(dtype, codes, 64, 64, 4, 2, [(context, draft), (context - 1, draft)], kind="chain", seed=draft)
+        c.scale = scale
+        c.v[0, 7], c.v[draft, 100] = math.inf, -math.inf
+        if not codes:
+            _spoil(c, 0, context - 1, math.inf)
+        _check(c, c.run())
