@@ -38,10 +38,10 @@ constexpr float LAZY = 8.f;
 // Values' exponents from which a weight times 2^-exponent is the probability: beside values of 2^40, what is lost is below 2^-30 of the largest
 constexpr int LOWEST = -63;
 
-// f * y for sums that are brought to a larger maximum.  An infinite value that a row sees counts whatever its weight is, so where the factor is zero in 32 bits
-// it stays what it is.
-__device__ __forceinline__ float rescaled(float f, float y) { return fabsf(y) < __builtin_inff() ? f * y : y; }
-__device__ __forceinline__ f32x4 rescaled(float f, f32x4 y) { return (f32x4){rescaled(f, y[0]), rescaled(f, y[1]), rescaled(f, y[2]), rescaled(f, y[3])}; }
+// The root of the factor by which what has been added up is brought from maximum m to m_new.  It is multiplied with twice: a sum of 2^100 (of values of zero) may
+// count where the whole factor is zero in 32 bits, and an infinite value that a row sees counts whatever its weight is (zero times it would be NaN; what is
+// finite is below 2^-124 after two times the least)
+__device__ __forceinline__ float root_of(float m, float m_new) { return fmaxf(__builtin_amdgcn_exp2f(0.5f * (m - m_new)), 0x1p-126f); }
 
 // Largest of the four lanes that share l15, by lane swaps (column_max goes through LDS: two latencies in every tile's chain)
 __device__ __forceinline__ float rows_max(float v) {

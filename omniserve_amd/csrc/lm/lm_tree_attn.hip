@@ -82,10 +82,10 @@ struct Tree {
         sum = ONE ? sum + x[u][r] : __builtin_fmaf(x[u][r], inv[u][r], sum);
       }
     if (__any(grows)) {
-      const float root = __builtin_amdgcn_exp2f(0.5f * (m_run[i] - m_new)), alpha = root * root;
-      l_run[i] = l_run[i] * root * root;      // (alpha may be too small where the sum, of 2^100 for values of zero, is not)
+      const float root = root_of(m_run[i], m_new);
+      l_run[i] = l_run[i] * root * root;
 #pragma unroll
-      for (int c = 0; c < NVB; ++c) acc[i][c] = rescaled(alpha, acc[i][c]);
+      for (int c = 0; c < NVB; ++c) acc[i][c] = acc[i][c] * root * root;
     }
     l_run[i] += low ? own : ONE ? sum * inv_all : sum;
     m_run[i] = m_new;
@@ -531,9 +531,9 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
       float sum = 0.f;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const float root = wl[w][rr] != 0.f ? __builtin_amdgcn_exp2f(0.5f * (wm[w][rr] - m)) : 0.f;
+        const float root = wl[w][rr] != 0.f ? root_of(wm[w][rr], m) : 0.f;
         sum += wl[w][rr] * root * root;
-        y += rescaled(root * root, *(const f32x4*)&res[w][rr][d]);
+        y += *(const f32x4*)&res[w][rr][d] * root * root;
       }
       if (!s.whole) {
         const int64_t at = part + 16 * i + rr;
@@ -583,7 +583,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p, int rows, i
     load(w);      // (beside the sums' request)
     const bool in = s0 + l < parts;
     const float ms = in ? p.ml[2 * (at0 + (s0 + l) * step)] : NEG, ls = in ? p.ml[2 * (at0 + (s0 + l) * step) + 1] : 0.f;
-    const float root = ls != 0.f ? __builtin_amdgcn_exp2f(0.5f * (ms - m)) : 0.f, f = root * root;
+    const float root = ls != 0.f ? root_of(ms, m) : 0.f;
     float t = ls * root * root;
 #pragma unroll
     for (int k = LR / 2; k > 0; k >>= 1) t += __shfl_xor(t, k, 64);
@@ -591,7 +591,10 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p, int rows, i
     const int end = min(LR, parts - s0);
     for (int s1 = w; s1 < end; s1 += 8 * waves) {
 #pragma unroll
-      for (int s = 0; s < 8; ++s) y += rescaled(s1 + s * waves < LR ? __shfl(f, lane - l + (s1 + s * waves) % LR, 64) : 0.f, v[s]);
+      for (int s = 0; s < 8; ++s) {
+        const float f = s1 + s * waves < LR ? __shfl(root, lane - l + (s1 + s * waves) % LR, 64) : 0.f;
+        y += v[s] * f * f;
+      }
       if (s1 + 8 * waves < end) load(s1 + 8 * waves);
     }
   }

@@ -217,10 +217,10 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
         else sum = __builtin_fmaf(x[u][r], inv[u][r], sum);
       }
     if (__any(grows)) {
-      const float root = __builtin_amdgcn_exp2f(0.5f * (m_run[i] - m_new)), alpha = root * root;
-      l_run[i] = l_run[i] * root * root;      // (alpha may be too small where the sum, of 2^100 for values of zero, is not)
+      const float root = root_of(m_run[i], m_new);
+      l_run[i] = l_run[i] * root * root;
 #pragma unroll
-      for (int c = 0; c < NVB; ++c) acc[i][c] = rescaled(alpha, acc[i][c]);
+      for (int c = 0; c < NVB; ++c) acc[i][c] = acc[i][c] * root * root;
     }
     l_run[i] += low ? own : one.value ? sum * inv_all : sum;
     m_run[i] = m_new;
