@@ -48,6 +48,26 @@ struct Tree {
 
   __device__ __forceinline__ Tree(const TreeArgs& a) : p(a) {}
 
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+#pragma unroll
+      for (int c = 0; c < NVB; ++c) acc[i][c] = zero4();
+      m_run[i] = NEG;
+      l_run[i] = 0.f;
+    }
+  }
+  __device__ __forceinline__ bool finite() const {      // are all sums of this wave?
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+      for (int c = 0; c < NVB; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z = __builtin_fmaf(acc[i][c][r], 0.f, z);
+    return !__any(z != 0.f);
+  }
+
   __device__ __forceinline__ void wave_sync() const {      // LDS operations of one wave are in order
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -436,11 +456,8 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
     for (int j = 0; j < T::CH; ++j)
 #pragma unroll
       for (int h = 0; h < T::PF; ++h) t.qf[i][j * T::PF + h] = r < R ? *(const frag_t*)(q + 64 * j + 16 * t.l4 + FR * h) : frag_t{};
-#pragma unroll
-    for (int c = 0; c < T::NVB; ++c) t.acc[i][c] = zero4();
-    t.m_run[i] = NEG;
-    t.l_run[i] = 0.f;
   }
+  t.clear();
 #pragma unroll
   for (int m = 1; m < 16; m <<= 1) {
     low_min = min(low_min, __shfl_xor(low_min, m, 64));
@@ -477,11 +494,19 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
         const int64_t at = ((int64_t)min(max(pg, 0), p.pages - 1) * p.G + g) * PAGE + tl * T::KT % PAGE;
         t.load_elems(c, kc + at * DK, DK, vc + at * DV, DV, T::KT);
       };
-      load(tile, page);
-      int ahead = tile + NW < tb ? bt[(tile + NW) / PER_PAGE] : 0;
-      for (; tile < tb; tile += NW) {
+      int ahead;
+      auto begin = [&]() {
+        tile = ta + wave;
+        page = bt[tile / PER_PAGE];
+        load(tile, page);
+        ahead = tile + NW < tb ? bt[(tile + NW) / PER_PAGE] : 0;
+      };
+      begin();
+      // An infinite value in a tile that all rows see whole passes through the products, where the second half of a weight, or a weight of zero, makes it NaN.  A
+      // wave whose sums are not finite goes over its tiles once more with such values taken out, as those of partly seen tiles always are.
+      for (bool careful = false; tile < tb;) {
         const int kb = tile * T::KT, hi = (uint32_t)page < (uint32_t)p.pages ? length - kb : 0, lo = max(k0 - kb, 0);
-        const bool edge = hi < T::KT || kb <= low_max;
+        const bool edge = careful || hi < T::KT || kb <= low_max;
         page = ahead;
         t.elem_tile(c, lo, hi, edge, [&](int i, int key) { return (bool)((int)(key >= lo) & (int)(key < hi) & (int)(kb + key > t.low[i])); },
                     [&]() {
@@ -489,6 +514,12 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
                       load(tile + NW, page);
                       ahead = tile + 2 * NW < tb ? bt[(tile + 2 * NW) / PER_PAGE] : 0;
                     });
+        tile += NW;
+        if (tile >= tb && !careful && !t.finite()) {
+          careful = true;
+          t.clear();
+          begin();
+        }
       }
     }
   }

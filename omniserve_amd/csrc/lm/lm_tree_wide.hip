@@ -57,7 +57,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l15 = lane & 15, l4 = lane >> 4;
   uint8_t* own = lds + W::NBUF * W::SLOT + wave * W::OWN;
   // smallest, largest of the rows' bounds; whether a context tile has non-finite values; a drafted tile, its largest value (words of their own: a wave may
-  // still have to read the last context tile's when another one clears them)
+  // still have to read the last context tile's when another one clears them); whether the sums have some
   int* shared = (int*)(lds + W::NBUF * W::SLOT + NW * W::OWN);
   const int r0 = s.rb * W::ROWS + wave * 16 * NR;
   const bool live = r0 < s.R;                                         // (a wave without rows fetches its pieces and waits with the others)
@@ -94,11 +94,14 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   const __attribute__((address_space(4))) int* bt = (const __attribute__((address_space(4))) int*)(uintptr_t)s.bt;
   auto page_of = [&](int t) { return t < tb ? bt[t / PER_PAGE] : 0; };
   int pages[W::NBUF];      // of tiles t, t + 1, ..
+  auto fetch_first = [&]() {
 #pragma unroll
-  for (int j = 0; j < W::NBUF; ++j) pages[j] = page_of(ta + j);
+    for (int j = 0; j < W::NBUF; ++j) pages[j] = page_of(ta + j);
 #pragma unroll
-  for (int j = 0; j < W::NBUF - 1; ++j)
-    if (ta + j < tb) fetch(ta + j, pages[j], j);
+    for (int j = 0; j < W::NBUF - 1; ++j)
+      if (ta + j < tb) fetch(ta + j, pages[j], j);
+  };
+  fetch_first();
 
   // ---- rows ----
   auto token_of = [&](int i) { return s.f0 + min(r0 + 16 * i + l15, s.R - 1) / s.gs; };
@@ -115,7 +118,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
     low_max = max(low_max, lo);
     low[i] = row_ok(i) ? lo : INT32_MAX;
   }
-  if (tid == 0) { shared[0] = INT32_MAX; shared[1] = INT32_MIN; }
+  if (tid == 0) { shared[0] = INT32_MAX; shared[1] = INT32_MIN; shared[5] = 0; }
   __syncthreads();
 #pragma unroll
   for (int m = 1; m < 16; m <<= 1) {
@@ -177,13 +180,16 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 
   f32x4 acc[NR][NVB];
   float m_run[NR], l_run[NR];
+  auto clear = [&]() {
 #pragma unroll
-  for (int i = 0; i < NR; ++i) {
+    for (int i = 0; i < NR; ++i) {
 #pragma unroll
-    for (int c = 0; c < NVB; ++c) acc[i][c] = zero4();
-    m_run[i] = NEG;
-    l_run[i] = 0.f;
-  }
+      for (int c = 0; c < NVB; ++c) acc[i][c] = zero4();
+      m_run[i] = NEG;
+      l_run[i] = 0.f;
+    }
+  };
+  clear();
   const float inv_scale = 1.0f / p.scale;
 
   // x: scores (with e / scale), unseen ones NEG -> weights; low: some exponent is below LOWEST
@@ -307,9 +313,10 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 
   // ---- the context ----
   int slot = 0;
-  for (int t = ta; t < tb; ++t) {
+  bool careful = false;      // (a second time over the tiles, where infinite elements may have become NaN: see the other kernel)
+  for (int t = ta; t < tb;) {
     const int kb = t * KT, page = pages[0], hi = (uint32_t)page < (uint32_t)p.pages ? s.length - kb : 0, lo = max(k0 - kb, 0);
-    const bool edge = hi < KT || kb <= low_max;
+    const bool edge = careful || hi < KT || kb <= low_max;
     if (W::NBUF > 2 && t + 1 < tb) wait_pieces<W::PIECES>();
     else wait_pieces<0>();
     __syncthreads();      // tile t is there; everyone has read the one before it
@@ -423,6 +430,26 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
         }
       }
     }
+    ++t;
+    if constexpr (!CODES)
+      if (t == tb && !careful) {
+        float z = 0.f;
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+          for (int c = 0; c < NVB; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z = __builtin_fmaf(acc[i][c][r], 0.f, z);
+        if (__any(z != 0.f) && lane == 0) atomicOr(&shared[5], 1);
+        __syncthreads();
+        if (shared[5] != 0) {
+          careful = true;
+          t = ta;
+          slot = 0;
+          clear();
+          fetch_first();
+        }
+      }
   }
 
   // ---- the drafted tokens ----

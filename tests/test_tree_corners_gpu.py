@@ -92,3 +92,18 @@ def test_an_infinite_value_of_no_weight(dtype, codes, context, draft):
         if not codes:
             _spoil(c, 0, context - 1, math.inf)
         _check(c, c.run())
+
+
+@pytest.mark.parametrize("draft", DRAFTS)
+@pytest.mark.parametrize("context,scale", [(300, None), (300, 8.0), (5000, None), (5000, 8.0)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_infinite_values_in_full_pages(dtype, context, scale, draft):
+    """Infinities of elements in pages that every row sees whole: the sum of such a row is infinite, of both signs NaN, and nothing else is touched"""
+    c = Case(dtype, False, 128, 64, 4, 2, [(context, draft), (context // 3, draft)], seed=draft)
+    c.scale = scale or c.scale
+    _spoil(c, 0, 3, math.inf, 0)
+    _spoil(c, 0, context // 2, -math.inf, 1)
+    _spoil(c, 0, 40, math.inf, 2)
+    _spoil(c, 0, context // 2 + 33, -math.inf, 2)
+    _spoil(c, 1, 20, math.nan, 9)
+    _check(c, c.run())
