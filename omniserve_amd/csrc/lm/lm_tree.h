@@ -88,6 +88,18 @@ __device__ __forceinline__ f16x8 code_halves(u32x2 w) {
   return f;
 }
 
+// Half h of 16 codes times a power of two, as an operand
+__device__ __forceinline__ frag_t code_frag(const u32x4& w, int h, float scale) {
+  frag_t f;
+#pragma unroll
+  for (int m = 0; m < FR / 4; ++m) {
+    const quad_t z = decode4(w[h * (FR / 4) + m], scale);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[4 * m + e] = z[e];
+  }
+  return f;
+}
+
 // w without its NaN codes (seven low bits ones); bad: there was one
 __device__ __forceinline__ uint32_t drop_nan_codes(uint32_t w, bool& bad) {
   const uint32_t nan = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;

@@ -154,17 +154,6 @@ struct Tree {
     }
   }
 
-  __device__ __forceinline__ static frag_t code_frag(const u32x4& w, int h, float scale) {
-    frag_t f;
-#pragma unroll
-    for (int m = 0; m < FR / 4; ++m) {
-      const quad_t z = decode4(w[h * (FR / 4) + m], scale);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f[4 * m + e] = z[e];
-    }
-    return f;
-  }
-
   // Scores of the tile's keys, and the next tile's request behind them; keys lo .. hi - 1 of the tile exist.
   template <typename Next>
   __device__ __forceinline__ void code_tile(Codes& c, int kb, int lo, int hi, bool edge, Next next) {

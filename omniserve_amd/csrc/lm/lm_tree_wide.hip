@@ -3,9 +3,9 @@
 //
 // Bound by the vector units beside the matrix units (a softmax weight costs 4 vector instructions, one of them an exponential of four times the
 // length, and 256 operations of the matrix units), so that what a weight does not need is done elsewhere:
-//   keys stay codes: the scaled MFMA takes them with their power of two.  A query row becomes TWO rows of codes, q = 2^e (hi + lo / 16): an element's
-//     8 significant bits are 4 and 4, and what is smaller than 2^-15 of the row's largest is off by at most 2^-21 of that.  Two products of 128 at
-//     twice the rate of bf16: as long as one, and no conversion;
+//   a key is decoded with its power of two into bf16, which holds it exactly.  (Products of the codes themselves, at twice the rate and without the decoding, take 175 us
+//     where this takes 205, but the matrix units add products of 8-bit floats in fewer than 32 bits: a sum of 128 was off by up to 2^-12 of its largest product, of
+//     bf16 by 2^-21);
 //   a value's exponent (lm_tree_attn.hip) is the products' initial accumulator, e / scale;
 //   2^-e and e / scale are formed by one lane per key and read back from LDS.
 // 4 trees of 64 over 32768 keys, 32 heads over 8: 174 us, 0.77 PFLOP/s; matrix units busy 36 % of the time, vector units 56, no LDS conflicts
@@ -14,7 +14,6 @@
 
 namespace lm {
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
@@ -40,7 +39,6 @@ struct Wide {
   static constexpr int KP = KBYTES / 1024, VP = VBYTES / 1024, EACH = (KP + VP + NW - 1) / NW, PIECES = EACH + (CODES ? 2 : 0);      // of a wave
   static constexpr int OWN = CODES ? 512 : 0;                                     // a wave's: keys' exponents
   static constexpr int LDS = NBUF * SLOT + NW * OWN + 64;
-  static constexpr int KS = CODES ? (DK + 127) / 128 : DK / 32;                  // steps of a key's product
   static constexpr float SHIFT = CODES ? 7.f : 0.f;                              // weights of codes are f16: at most 2^(LAZY + 7)
   typedef Tile<2 * DV> VT;
   typedef Tile<2 * DK> KTile;
@@ -132,50 +130,12 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   const int k0 = max(low_min, -1) + 1;
 
   // ---- queries ----
-  i32x8 qc[NR][2][CODES ? W::KS : 1];      // codes: hi, lo
-  int qe[NR][2];                           // their exponent bytes
-  frag_t qf[NR][CODES ? 1 : W::KS];
+  frag_t qf[NR][DK / 32];      // (of codes: the order that half a slot of 16 codes has)
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     const elem_t* qrow = query_of(i);
-    if constexpr (CODES) {
-      float y[W::KS][32], top = 0.f;
 #pragma unroll
-      for (int k = 0; k < W::KS; ++k)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const frag_t f = row_ok(i) && 128 * k + 64 * j < DK ? *(const frag_t*)(qrow + 128 * k + 64 * j + 16 * l4 + 8 * h) : frag_t{};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              y[k][16 * j + 8 * h + e] = (float)f[e];
-              const float m = fabsf((float)f[e]);
-              top = m < __builtin_inff() ? fmaxf(top, m) : top;
-            }
-          }
-      const int e = row_exponent(column_max(top));
-      qe[i][0] = e + 127;
-      qe[i][1] = e + 123;
-#pragma unroll
-      for (int k = 0; k < W::KS; ++k)
-#pragma unroll
-        for (int w = 0; w < 8; ++w) {
-          // (within 448 all of them: no bounds; z - z makes the second code of NaN and infinities NaN)
-          const float f = pow2(-e), *v = &y[k][4 * w], z[4] = {v[0] * f, v[1] * f, v[2] * f, v[3] * f};
-          const uint32_t hi = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false), true);
-          const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, 1.0f, true);
-          const float back[4] = {a[0], a[1], b[0], b[1]};
-          float rest[4];
-#pragma unroll
-          for (int m = 0; m < 4; ++m) rest[m] = __builtin_fmaf(16.f, z[m] - back[m], z[m] - z[m]);
-          qc[i][0][k][w] = (int)hi;
-          qc[i][1][k][w] = __builtin_amdgcn_cvt_pk_fp8_f32(rest[2], rest[3], __builtin_amdgcn_cvt_pk_fp8_f32(rest[0], rest[1], 0, false), true);
-        }
-    } else {
-#pragma unroll
-      for (int k = 0; k < W::KS; ++k) qf[i][k] = row_ok(i) ? *(const frag_t*)(qrow + 32 * k + 8 * l4) : frag_t{};
-    }
+    for (int k = 0; k < DK / 32; ++k) qf[i][k] = row_ok(i) ? *(const frag_t*)(qrow + (CODES ? 64 * (k >> 1) + 16 * l4 + 8 * (k & 1) : 32 * k + 8 * l4)) : frag_t{};
   }
 
   f32x4 acc[NR][NVB];
@@ -370,22 +330,17 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
         for (int u = 0; u < NU; ++u) {
           const f32x4 ev = mine[4 * u + l4];
           inv[u] = mine[16 + 4 * u + l4];
-          const int ke = exps[16 * u + l15];
+          const float scale = scale_of(exps[16 * u + l15]);
 #pragma unroll
-          for (int k = 0; k < W::KS; ++k) {
-            i32x8 kf = {};
+          for (int j = 0; j < DK / 64; ++j) {
+            const int row = 16 * u + l15;
+            const u32x4 w = *(const u32x4*)(kt + row * DK + (((4 * j + l4) ^ key_swizzle<DK>(row)) << 4));
 #pragma unroll
-            for (int j = 0; j < 2 && 128 * k + 64 * j < DK; ++j) {
-              const int row = 16 * u + l15;
-              const i32x4 w = *(const i32x4*)(kt + row * DK + (((8 * k + 4 * j + l4) ^ key_swizzle<DK>(row)) << 4));
+            for (int h = 0; h < 2; ++h) {
+              const frag_t kf = code_frag(w, h, scale);
 #pragma unroll
-              for (int m = 0; m < 4; ++m) kf[4 * j + m] = w[m];
+              for (int i = 0; i < NR; ++i) x[i][u] = mma(kf, qf[i][2 * j + h], j == 0 && h == 0 ? ev : x[i][u]);
             }
-#pragma unroll
-            for (int i = 0; i < NR; ++i)
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                x[i][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, qc[i][h][k], h == 0 && k == 0 ? ev : x[i][u], 0, 0, 0, ke, 0, qe[i][h]);
           }
         }
 #pragma unroll

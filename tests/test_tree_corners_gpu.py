@@ -107,3 +107,21 @@ def test_infinite_values_in_full_pages(dtype, context, scale, draft):
     _spoil(c, 0, context // 2 + 33, -math.inf, 2)
     _spoil(c, 1, 20, math.nan, 9)
     _check(c, c.run())
+
+
+@pytest.mark.parametrize("draft", DRAFTS)
+@pytest.mark.parametrize("dk", [64, 128, 256])
+@pytest.mark.parametrize("codes", [True, False])
+def test_scores_are_summed_in_32_bits(codes, dk, draft):
+    """Queries and keys with a few channels much larger than the others, of either sign: the largest products cancel or outweigh the rest, which counts all the same"""
+    c = Case(BF16, codes, dk, 64, 4, 2, [(500, draft), (70, draft)], seed=draft + dk)
+    q, k = c.q.view(-1, 4, dk), c.k.view(-1, 2, dk)
+    q[..., [0, 7, dk - 1]] *= 30
+    k[..., [0, 7, dk - 1]] *= 8
+    if codes:
+        c.cache[0][..., [0, 7, dk - 1]] = torch.where(c.cache[0][..., [0, 7, dk - 1]] > 127, 0xf6, 0x76).to(torch.uint8)
+    n = c.q.shape[0]
+    ref = attention(c.q.double().view(n, c.H, dk), c.k.double().view(n, c.G, dk), c.v.double().view(n, c.G, 64), c.mask, c.first.cpu(), c.pos, *c.pools(), c.bt, c.length, c.scale,
+                    NO_WINDOW, c.max_draft, 2)
+    over = (c.run().double().view(n, 4, 64) - ref[0]).abs() / attention_bound(BF16, codes, dk, *ref[:5], 0.0)      # (no term for queries in codes)
+    assert float(over.max()) <= 1.0, float(over.max())
