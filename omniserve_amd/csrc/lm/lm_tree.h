@@ -50,6 +50,22 @@ __device__ __forceinline__ float rows_max(float v) {
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
+template <int C>
+struct Dpp { static constexpr int value = C; };
+// Largest of N neighbouring lanes, 8 to 32 (lane swaps inside a row of 16, then of two rows)
+template <int N>
+__device__ __forceinline__ float lanes_max(float v) {
+  auto with = [&](auto ctrl) { v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, false))); };
+  with(Dpp<0xb1>());       // lane ^ 1
+  with(Dpp<0x4e>());       // lane ^ 2
+  with(Dpp<0x141>());      // the other four of eight
+  if constexpr (N > 8) with(Dpp<0x140>());
+  if constexpr (N > 16) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  }
+  return v;
+}
 // x in a place that few tiles come to: nothing formed from it moves in front of the branch
 __device__ __forceinline__ int here(int x) {
   asm volatile("" : "+v"(x));

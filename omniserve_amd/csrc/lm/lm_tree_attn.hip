@@ -14,8 +14,8 @@
 // Codes (lm_kv_codes.h).  A key's power of two scales its operand in the conversion.  A value's, 2^e, joins the softmax: with weights
 // w_j = 2^(s_j + e_j - m'), m' the running maximum of s_j + e_j, the outputs are sum w_j code_j and the sum of the probabilities is
 // sum w_j 2^(-e_j).  So w_j is at most 2^LAZY and is ONE f16 operand (11 bits, times 2^7 so that small ones stay normal) beside codes that f16
-// holds exactly; bf16 values need two bf16 operands for theirs (16 bits).  The drafted values, whose exponents nothing has taken out, are
-// divided by a power of two of their own.  A tile with rows of very small values, or none but zeros (2^-100), beside which the others' maximum leaves
+// holds exactly; bf16 values need two bf16 operands for theirs (16 bits).  A drafted token's values are divided by such a power of two of their own first, so
+// that nothing depends on the size of values that a row does not see.  A tile with rows of very small values, or none but zeros (2^-100), beside which the others' maximum leaves
 // such a weight nothing, multiplies its roots with 2^(-e) one by one: its rows count in the sum as all others do.
 #include "lm_tree.h"
 #include "omniserve_lm.h"
@@ -34,11 +34,13 @@ struct Tree {
   static constexpr int KT = CODES ? 64 : 32, NU = KT / 16;        // keys of a context tile
   static constexpr int STAGE = 64 * DV;                           // bytes of a wave's V tile: 64 rows of codes, 32 of bf16
   static constexpr int NW = 4;                                    // waves
-  static constexpr int RED = NW * 16 * (DV + 4) * 4, LDS = SPLIT && NW * STAGE > RED ? NW * STAGE : RED;
+  static constexpr int EXPS = 256;                                // behind the V tiles, a wave's: exponents of 32 drafted values and 2^-exponent
+  static constexpr int RED = NW * 16 * (DV + 4) * 4, LDS = SPLIT && NW * (STAGE + EXPS) > RED ? NW * (STAGE + EXPS) : RED;
   typedef Tile<SPLIT ? DV * 2 : 256> VT;
 
   const TreeArgs& p;
   uint8_t* stage;                   // this wave's part of the LDS
+  float* exps;
   int lane, l15, l4;
   frag_t qf[NR][NKF];
   f32x4 acc[NR][NVB];
@@ -73,9 +75,10 @@ struct Tree {
     __builtin_amdgcn_wave_barrier();
   }
 
-  // x: scores times scale plus the values' exponents, unseen ones NEG; inv: 2^-exponent; low: some exponent is below LOWEST.  Leaves the weights in x.
+  // x: scores times scale plus the values' exponents, unseen ones NEG; inv: 2^-exponent (ONE: there are none); low: some exponent is below LOWEST.  Leaves the
+  // weights in x.
   template <int U, bool ONE>
-  __device__ __forceinline__ void softmax(int i, f32x4 (&x)[U], const f32x4 (&inv)[U], float inv_all, bool low) {
+  __device__ __forceinline__ void softmax(int i, f32x4 (&x)[U], const f32x4 (&inv)[U], bool low) {
     float t = NEG;
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -85,13 +88,13 @@ struct Tree {
     const bool grows = t > m_run[i] + (low ? 0.f : LAZY);      // (the first key's always; a NaN never)
     const float m_new = grows ? t : m_run[i], m_sub = (m_new <= NEG ? 0.f : m_new) - SHIFT;
     float own = 0.f, sum = 0.f;
-    if (low) {
+    if (!ONE && low) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float root = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][r], 0.5f, -0.5f * m_sub));
-          own = __builtin_fmaf(root * (ONE ? inv_all : inv[u][r]), root, own);
+          own = __builtin_fmaf(root * inv[u][r], root, own);
         }
     }
 #pragma unroll
@@ -107,7 +110,7 @@ struct Tree {
 #pragma unroll
       for (int c = 0; c < NVB; ++c) acc[i][c] = acc[i][c] * root * root;
     }
-    l_run[i] += low ? own : ONE ? sum * inv_all : sum;
+    l_run[i] += low ? own : sum;
     m_run[i] = m_new;
   }
 
@@ -236,7 +239,7 @@ struct Tree {
             x[i][u][r] = (int)(key >= lo) & (int)(key < hi) & (int)(kb + key > low[i]) ? x[i][u][r] : NEG;
           }
       }
-      softmax<NU, false>(i, x[i], inv, 1.f, low_values);
+      softmax<NU, false>(i, x[i], inv, low_values);
       if constexpr (SPLIT) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) pq[i][u] = (f16x4){(_Float16)x[i][u][0], (_Float16)x[i][u][1], (_Float16)x[i][u][2], (_Float16)x[i][u][3]};
@@ -323,15 +326,21 @@ struct Tree {
         for (int s = 0; s < NKF; ++s) x[i][u] = mma(c.k[u][s], qf[i][s], x[i][u]);
       }
     bool bad = false;
-    int e = 0;
     const elem_t* vp = c.vp;
     const int64_t ldv = c.ldv;
+    f32x4 ev[2], inv[2];      // of this lane's keys, as those of codes
     if constexpr (SPLIT) {
+      float of[CODES ? DV / 16 : 1];      // exponents of the rows that this lane has a part of
       if (edge) {
-        float top = 0.f;
 #pragma unroll
         for (int i = 0; i < DV / 16; ++i) {
+          if (64 * i / (DV / 8) >= hi) {      // (a step without drafts has one row)
+            c.v[i] = frag_t{};
+            if constexpr (CODES) of[i] = 0.f;
+            continue;
+          }
           const int row = (64 * i + lane) / (DV / 8);
+          float top = 0.f;
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             float y = row >= lo && row < hi ? (float)c.v[i][k] : 0.f;
@@ -341,36 +350,68 @@ struct Tree {
             top = fmaxf(top, fabsf(y));
             c.v[i][k] = (elem_t)y;
           }
-        }
-        bad = __any(bad);
-        if constexpr (CODES) {
-#pragma unroll
-          for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-          e = row_exponent(top);
-          const float f = pow2(-e);
-#pragma unroll
-          for (int i = 0; i < DV / 16; ++i)
+          if constexpr (CODES) {
+            const int e = row >= lo && row < hi ? row_exponent(lanes_max<DV / 8>(top)) : 0;
+            const float f = pow2(-e);
+            of[i] = (float)e;
 #pragma unroll
             for (int k = 0; k < 8; ++k) c.v[i][k] = (elem_t)((float)c.v[i][k] * f);
+          }
         }
+        bad = __any(bad);
       }
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int i = 0; i < DV / 16; ++i) {
         const int at = 64 * i + lane;
         *(frag_t*)(stage + VT::slot(at / VT::NS, at % VT::NS)) = c.v[i];
+        if constexpr (CODES)
+          if (at % VT::NS == 0) {
+            exps[at / VT::NS] = of[i];
+            exps[32 + at / VT::NS] = pow2(-(int)of[i]);
+          }
       }
+    } else if constexpr (CODES) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = 16 * s + 4 * l4 + r;
+          float top = 0.f;
+#pragma unroll
+          for (int cb = 0; cb < NVB; ++cb) {
+            const float m = fabsf((float)vp[min(key, c.rows - 1) * ldv + 16 * cb + l15]);
+            top = m < __builtin_inff() ? fmaxf(top, m) : top;
+          }
+          const int e = key >= lo && key < hi ? row_exponent(lanes_max<16>(top)) : 0;
+          ev[s][r] = (float)e;
+          inv[s][r] = pow2(-e);
+        }
     }
     next();
     if constexpr (SPLIT) wave_sync();
-    const float ev = (float)e;
+    if constexpr (SPLIT && CODES) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        ev[u] = *(const f32x4*)&exps[16 * u + 4 * l4];
+        inv[u] = *(const f32x4*)&exps[32 + 16 * u + 4 * l4];
+      }
+    }
+    bool low_values = false;
+    if constexpr (CODES) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) low_values |= inv[u][r] > pow2(-LOWEST);
+      low_values = __any(low_values);
+    }
     quad_t pq[NR][2][NOPND];
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[i][u][r] = __builtin_fmaf(x[i][u][r], p.scale, ev);
+        for (int r = 0; r < 4; ++r) x[i][u][r] = CODES ? __builtin_fmaf(x[i][u][r], p.scale, ev[u][r]) : x[i][u][r] * p.scale;
       if (edge) {
         const int key = here(4 * l4);
 #pragma unroll
@@ -378,7 +419,7 @@ struct Tree {
 #pragma unroll
           for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, key + 16 * u + r) ? x[i][u][r] : NEG;
       }
-      softmax<2, true>(i, x[i], x[i], pow2(-e), e < LOWEST);
+      softmax<2, !CODES>(i, x[i], inv, low_values);
 #pragma unroll
       for (int u = 0; u < 2; ++u) split_quad(x[i][u], pq[i][u]);
     }
@@ -400,6 +441,7 @@ struct Tree {
               const bool fine = fabsf(y) < __builtin_inff();
               bad |= !fine;
               y = fine ? y : 0.f;
+              if constexpr (CODES) y *= inv[s][r];
             }
             v[s][r] = (elem_t)y;
           }
@@ -430,6 +472,7 @@ __global__ __launch_bounds__(256, NR == 1 && DK + DV <= 256 ? 2 : 1) void tree_a
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   t.lane = tid & 63; t.l15 = tid & 15; t.l4 = t.lane >> 4;
   t.stage = lds + wave * (SPLIT ? T::STAGE : 0);
+  t.exps = (float*)(lds + T::NW * T::STAGE + wave * T::EXPS);      // (SPLIT alone uses it)
   int low_min = INT32_MAX, low_max = INT32_MIN, token[NR];
 #pragma unroll
   for (int i = 0; i < NR; ++i) {

@@ -54,8 +54,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   if (!piece_of<KT, W::ROWS>(p, s, part)) return;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l15 = lane & 15, l4 = lane >> 4;
   uint8_t* own = lds + W::NBUF * W::SLOT + wave * W::OWN;
-  // smallest, largest of the rows' bounds; whether a context tile has non-finite values; a drafted tile, its largest value (words of their own: a wave may
-  // still have to read the last context tile's when another one clears them); whether the sums have some
+  // smallest, largest of the rows' bounds; whether a context tile has non-finite values; whether a drafted tile had some (a word of its own that nobody clears: a
+  // wave may still have to read what another one would clear); whether the sums have some
   int* shared = (int*)(lds + W::NBUF * W::SLOT + NW * W::OWN);
   const int r0 = s.rb * W::ROWS + wave * 16 * NR;
   const bool live = r0 < s.R;                                         // (a wave without rows fetches its pieces and waits with the others)
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
     low_max = max(low_max, lo);
     low[i] = row_ok(i) ? lo : INT32_MAX;
   }
-  if (tid == 0) { shared[0] = INT32_MAX; shared[1] = INT32_MIN; shared[5] = 0; }
+  if (tid == 0) { shared[0] = INT32_MAX; shared[1] = INT32_MIN; shared[3] = shared[4] = 0; }
   __syncthreads();
 #pragma unroll
   for (int m = 1; m < 16; m <<= 1) {
@@ -152,8 +152,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   clear();
   const float inv_scale = 1.0f / p.scale;
 
-  // x: scores (with e / scale), unseen ones NEG -> weights; low: some exponent is below LOWEST
-  auto softmax = [&](int i, auto& x, const auto& inv, auto one, float inv_all, bool low) {
+  // x: scores (with e / scale), unseen ones NEG -> weights; inv: 2^-e (one: there are none); low: some exponent is below LOWEST
+  auto softmax = [&](int i, auto& x, const auto& inv, auto one, bool low) {
     constexpr int U = sizeof(x) / sizeof(f32x4);
     float t = NEG;
 #pragma unroll
@@ -165,13 +165,13 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
     const bool grows = t > m_run[i] + (low ? 0.f : LAZY);      // (the first key's always; a NaN never)
     const float m_new = grows ? t : m_run[i], m_sub = (m_new <= NEG ? 0.f : m_new) - W::SHIFT;
     float own = 0.f, sum = 0.f;
-    if (low) {
+    if (!one.value && low) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float root = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][r], 0.5f * p.scale, -0.5f * m_sub));
-          own = __builtin_fmaf(root * (one.value ? inv_all : inv[u][r]), root, own);
+          own = __builtin_fmaf(root * inv[u][r], root, own);
         }
     }
 #pragma unroll
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
       for (int c = 0; c < NVB; ++c) acc[i][c] = acc[i][c] * root * root;
     }
-    l_run[i] += low ? own : one.value ? sum * inv_all : sum;
+    l_run[i] += low ? own : sum;
     m_run[i] = m_new;
   };
   auto wave_sync = [&]() {
@@ -210,8 +210,9 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
         }
     }
   };
-  // A tile of 32 keys and values in elements at `tile`: products, weights, products
-  auto elem_products = [&](const uint8_t* kt, const uint8_t* vt, const frag_t (&q)[NR][DK / 32], bool edge, bool bad, int e, int lo, int hi, auto seen, auto value) {
+  // A tile of 32 keys and values in elements: products, weights, products; ev, inv: e / scale and 2^-e of a codes' kernel's drafted values, as those of codes
+  auto elem_products = [&](const uint8_t* kt, const uint8_t* vt, const frag_t (&q)[NR][DK / 32], bool edge, bool bad, const f32x4 (&ev)[2], const f32x4 (&inv)[2], bool low_values, int lo,
+                           int hi, auto seen, auto value) {
     f32x4 x[NR][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       for (int k = 0; k < DK / 32; ++k) {
         const frag_t kf = W::KTile::frag(kt, 16 * u + l15, 4 * k + l4);
 #pragma unroll
-        for (int i = 0; i < NR; ++i) x[i][u] = mma(kf, q[i][k], k == 0 ? (f32x4)((float)e * inv_scale) : x[i][u]);
+        for (int i = 0; i < NR; ++i) x[i][u] = mma(kf, q[i][k], k > 0 ? x[i][u] : CODES ? ev[u] : zero4());
       }
     quad_t pq[NR][2][2];
 #pragma unroll
@@ -231,7 +232,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, key + 16 * u + r) ? x[i][u][r] : NEG;
       }
-      softmax(i, x[i], x[i], Yes(), pow2(-e), e < LOWEST);
+      if constexpr (CODES) softmax(i, x[i], inv, No(), low_values);
+      else softmax(i, x[i], inv, Yes(), false);
 #pragma unroll
       for (int u = 0; u < 2; ++u) split_quad(x[i][u], pq[i][u]);
     }
@@ -294,7 +296,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       if (edge) bad = clean_elems(vt, lo, hi);
       if (live) {
         const elem_t* vb = (const elem_t*)p.vc + at * DV;
-        elem_products(kt, vt, qf, edge, bad, 0, lo, min(hi, KT), seen, [&](int j, int d) { return (float)vb[j * DV + d]; });
+        const f32x4 none[2] = {};
+        elem_products(kt, vt, qf, edge, bad, none, none, false, lo, min(hi, KT), seen, [&](int j, int d) { return (float)vb[j * DV + d]; });
       }
     } else {
       uint8_t* exps = vt + W::VBYTES;
@@ -364,7 +367,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
               for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, key + 16 * u + r) ? x[i][u][r] : NEG;
           }
-          softmax(i, x[i], inv, No(), 1.f, low_values);
+          softmax(i, x[i], inv, No(), low_values);
 #pragma unroll
           for (int u = 0; u < NU; ++u) pq[i][u] = (f16x4){(_Float16)x[i][u][0], (_Float16)x[i][u][1], (_Float16)x[i][u][2], (_Float16)x[i][u][3]};
         }
@@ -395,9 +398,9 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
           for (int c = 0; c < NVB; ++c)
 #pragma unroll
             for (int r = 0; r < 4; ++r) z = __builtin_fmaf(acc[i][c][r], 0.f, z);
-        if (__any(z != 0.f) && lane == 0) atomicOr(&shared[5], 1);
+        if (__any(z != 0.f) && lane == 0) atomicOr(&shared[4], 1);
         __syncthreads();
-        if (shared[5] != 0) {
+        if (shared[4] != 0) {
           careful = true;
           t = ta;
           slot = 0;
@@ -422,12 +425,11 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       const int64_t row0 = s.f0 + j0;
       uint8_t* kt = lds;
       uint8_t* vt = lds + E::KBYTES;
-      // Values pass through registers: non-finite ones are left out, codes' kernels divide by a power of two
+      // Values pass through registers: non-finite ones are left out, and beside codes a token's are divided by a power of two of their own
       constexpr int VF = (32 * DV / 8 + 64 * NW - 1) / (64 * NW);
-      if (tid == 0) { shared[3] = 0; shared[4] = 0; }
+      float* exps = (float*)(lds + W::NBUF * W::SLOT);      // e / scale, from 64 on 2^-e (beside codes: the first wave's own)
       frag_t vf[VF];
       bool bad = false;
-      float top = 0.f;
 #pragma unroll
       for (int k = 0; k < VF; ++k) {
         const int i = tid + 64 * NW * k, row = i / (DV / 8), c = i % (DV / 8);
@@ -439,7 +441,9 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
         *(frag_t*)(kt + W::KTile::slot(row, c)) = *(const frag_t*)(p.k + (row0 + min(row, rows - 1)) * p.ldk + (int64_t)s.g * DK + 8 * c);
       }
 #pragma unroll
-      for (int k = 0; k < VF; ++k)
+      for (int k = 0; k < VF; ++k) {
+        const int i = tid + 64 * NW * k, row = i / (DV / 8), c = i % (DV / 8);
+        float top = 0.f;
 #pragma unroll
         for (int m = 0; m < 8; ++m) {
           const float y = (float)vf[k][m];
@@ -448,32 +452,38 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
           vf[k][m] = fine ? vf[k][m] : (elem_t)0.f;
           top = fine ? fmaxf(top, fabsf(y)) : top;
         }
-      if constexpr (CODES) {
+        if constexpr (CODES) {
+          const int e = row < rows ? row_exponent(lanes_max<DV / 8>(top)) : 0;
+          const float f = pow2(-e);
 #pragma unroll
-        for (int m = 32; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-        if (lane == 0) atomicMax(&shared[4], (int)__float_as_uint(top));      // (not negative: ordered like whole numbers)
+          for (int m = 0; m < 8; ++m) vf[k][m] = (elem_t)((float)vf[k][m] * f);
+          if (row < 32 && c == 0) {
+            exps[row] = (float)e * inv_scale;
+            exps[64 + row] = f;
+          }
+        }
+        if (row < 32) *(frag_t*)(vt + W::VT::slot(row, c)) = vf[k];
       }
       if (__any(bad) && lane == 0) atomicOr(&shared[3], 1);
       __syncthreads();
-      bad = shared[3] != 0;
-      const int e = CODES ? row_exponent(__uint_as_float((uint32_t)shared[4])) : 0;
-      const float f = pow2(-e);
-#pragma unroll
-      for (int k = 0; k < VF; ++k) {
-        const int i = tid + 64 * NW * k, row = i / (DV / 8), c = i % (DV / 8);
-        if constexpr (CODES)
-#pragma unroll
-          for (int m = 0; m < 8; ++m) vf[k][m] = (elem_t)((float)vf[k][m] * f);
-        if (row < 32) *(frag_t*)(vt + W::VT::slot(row, c)) = vf[k];
-      }
-      __syncthreads();
+      bad = shared[3] != 0;      // (of this tile or one before: then this one is looked through for nothing)
       if (!live) continue;
       uint32_t bits[NR];
 #pragma unroll
       for (int i = 0; i < NR; ++i)
         bits[i] = row_ok(i) && (j0 >> 6) < p.words ? (uint32_t)(p.mask[(int64_t)token_of(i) * p.words + (j0 >> 6)] >> (j0 & 63)) : 0u;
+      f32x4 ev[2] = {}, inv[2] = {};
+      bool low_values = false;
+      if constexpr (CODES) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          ev[u] = *(const f32x4*)&exps[16 * u + 4 * l4];
+          inv[u] = *(const f32x4*)&exps[64 + 16 * u + 4 * l4];
+        }
+        low_values = __any(exps[64 + (lane & 31)] > pow2(-LOWEST));
+      }
       const elem_t* vb = p.v + row0 * p.ldv + (int64_t)s.g * DV;
-      elem_products(kt, vt, q, true, bad, e, 0, rows,
+      elem_products(kt, vt, q, true, bad, ev, inv, low_values, 0, rows,
                     [&](int i, int key) {
                       return (bool)((int)(key < rows) & (int)(bits[i] >> key & 1) & (int)(p.pos[min((int)row0 + key, s.f0 + s.drafted - 1)] > low[i]));
                     },

@@ -125,3 +125,38 @@ def test_scores_are_summed_in_32_bits(codes, dk, draft):
                     NO_WINDOW, c.max_draft, 2)
     over = (c.run().double().view(n, 4, 64) - ref[0]).abs() / attention_bound(BF16, codes, dk, *ref[:5], 0.0)      # (no term for queries in codes)
     assert float(over.max()) <= 1.0, float(over.max())
+
+
+@pytest.mark.parametrize("loud", [2.0 ** 16, 2.0 ** 40, 2.0 ** 100, 2.0 ** 120])
+@pytest.mark.parametrize("draft", [2, 12, 20, 64, 150])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_loud_drafted_value_is_its_own_affair(dtype, draft, loud):
+    """A drafted token of large values, and one of tiny ones, in the same tile as tokens that do not see them, or hardly"""
+    for kind in ("tree", "chain"):
+        c = Case(dtype, True, 64, 128, 4, 2, [(200, draft), (1500, draft), (0, draft)], kind=kind, seed=draft)
+        q, k = c.q.view(-1, 4, 64), c.k.view(-1, 2, 64)
+        q[..., 0] = 8
+        for b in range(3):
+            f0, at = int(c.first[b]), draft // 2
+            c.v[f0 + at] *= loud
+            c.v[f0 + draft - 1] /= loud
+            if b == 1:      # those who see it do so faintly
+                k[f0 + at, :, 0] = -40
+                continue
+            bit = 1 << at % 64
+            c.mask[[f0 + i for i in range(draft) if i != at], at // 64] &= ~(bit - (1 << 64) if bit >> 63 else bit)
+        _check(c, c.run())
+
+
+def test_a_drafted_value_of_every_size():
+    """Every drafted value has a power of two of its own, from the smallest to the largest, and none sees another"""
+    for draft in (7, 32, 150):
+        c = Case(BF16, True, 64, 64, 2, 1, [(130, draft)], seed=draft)
+        e = torch.linspace(-60, 120, draft, device=dev()).round()
+        c.v = (c.v.float().clamp(-4, 4) * torch.exp2(e)[:, None]).to(BF16)
+        i = torch.arange(draft)
+        c.mask.zero_()
+        c.mask[i, i // 64] = torch.ones(draft, dtype=torch.int64, device=dev()) << (i % 64).to(dev())
+        _check(c, c.run())
+        c.length.zero_()
+        _check(c, c.run())
