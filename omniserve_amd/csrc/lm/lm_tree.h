@@ -35,13 +35,27 @@ __device__ __forceinline__ int bound_of(const TreeArgs& p, int pos) { return p.w
 // A row's weights are relative to a maximum that is followed only when it has grown by so much (in powers of two): what has been added up is rescaled in a
 // few tiles, not in every second one
 constexpr float LAZY = 8.f;
-// Values' exponents from which a weight times 2^-exponent is the probability: beside values of 2^40, what is lost is below 2^-30 of the largest
-constexpr int LOWEST = -63;
+// A weight is 2^(s + e - m'), and a probability it times 2^-e, so that a weight may be too small for 32 bits whose probability is not: where a tile has exponents
+// SPREAD below that of the keys which have set the maximum, or below LOWEST (the sum of many probabilities, each 2^-e times a weight, could pass 32
+// bits), the weights' roots are multiplied with 2^-e one by one.  What is lost otherwise is below 2^-30 of the largest probability.
+constexpr int LOWEST = -63, SPREAD = 96;
 
 // The root of the factor by which what has been added up is brought from maximum m to m_new.  It is multiplied with twice: a sum of 2^100 (of values of zero) may
 // count where the whole factor is zero in 32 bits, and an infinite value that a row sees counts whatever its weight is (zero times it would be NaN; what is
 // finite is below 2^-124 after two times the least)
 __device__ __forceinline__ float root_of(float m, float m_new) { return fmaxf(__builtin_amdgcn_exp2f(0.5f * (m - m_new)), 0x1p-126f); }
+
+// Which tiles those are, of one wave.  Exponents are looked at as 2^-e.
+struct Loudness {
+  float loudest, limit;      // of the keys that have set a maximum; of the tiles that go without roots
+  __device__ __forceinline__ Loudness() : loudest(__builtin_inff()), limit(pow2(-LOWEST)) {}
+  __device__ __forceinline__ bool quiet(float most) const { return __any(most > limit); }      // most: the largest of this lane's
+  // a tile sets a row's maximum; least: the smallest of all its keys'
+  __device__ __forceinline__ void set(float least) {
+    loudest = fminf(loudest, least);
+    limit = fminf(pow2(-LOWEST), loudest * pow2(SPREAD));
+  }
+};
 
 // Largest of the four lanes that share l15, by lane swaps (column_max goes through LDS: two latencies in every tile's chain)
 __device__ __forceinline__ float rows_max(float v) {

@@ -45,6 +45,7 @@ struct Tree {
   frag_t qf[NR][NKF];
   f32x4 acc[NR][NVB];
   float m_run[NR], l_run[NR];
+  Loudness loud;
   int low[NR];                      // the newest position that the row does not see any more
   bool row_ok[NR];
 
@@ -75,18 +76,30 @@ struct Tree {
     __builtin_amdgcn_wave_barrier();
   }
 
-  // x: scores times scale plus the values' exponents, unseen ones NEG; inv: 2^-exponent (ONE: there are none); low: some exponent is below LOWEST.  Leaves the
-  // weights in x.
+  // x: scores times scale plus the values' exponents, unseen ones NEG; inv: 2^-exponent (ONE: there are none), most: the largest of this lane's.  Leaves the weights
+  // in x.
   template <int U, bool ONE>
-  __device__ __forceinline__ void softmax(int i, f32x4 (&x)[U], const f32x4 (&inv)[U], bool low) {
+  __device__ __forceinline__ void softmax(int i, f32x4 (&x)[U], const f32x4 (&inv)[U], float most) {
     float t = NEG;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int r = 0; r < 4; ++r) t = fmaxf(t, x[u][r]);
     t = rows_max(t);
+    bool low = !ONE && loud.quiet(most);
     const bool grows = t > m_run[i] + (low ? 0.f : LAZY);      // (the first key's always; a NaN never)
+    const bool some = __any(grows);
     const float m_new = grows ? t : m_run[i], m_sub = (m_new <= NEG ? 0.f : m_new) - SHIFT;
+    if constexpr (!ONE)
+      if (some) {
+        float least = inv[0][0];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) least = fminf(least, inv[u][r]);
+        loud.set(-rows_max(-least));
+        low = loud.quiet(most);
+      }
     float own = 0.f, sum = 0.f;
     if (!ONE && low) {
 #pragma unroll
@@ -104,7 +117,7 @@ struct Tree {
         x[u][r] = __builtin_amdgcn_exp2f(x[u][r] - m_sub);
         sum = ONE ? sum + x[u][r] : __builtin_fmaf(x[u][r], inv[u][r], sum);
       }
-    if (__any(grows)) {
+    if (some) {
       const float root = root_of(m_run[i], m_new);
       l_run[i] = l_run[i] * root * root;
 #pragma unroll
@@ -195,10 +208,11 @@ struct Tree {
     for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int r = 0; r < 4; ++r) { ev[u][r] = exponent_of(c.vx[u], r); inv[u][r] = inverse_of(c.vx[u], r); }
-    uint32_t high = ~0u;      // a byte's highest bit: it is 64 at least
+    float most = inv[0][0];
 #pragma unroll
-    for (int u = 0; u < NU; ++u) high &= c.vx[u] | c.vx[u] << 1;
-    const bool low_values = __any(~high & 0x80808080u);
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) most = fmaxf(most, inv[u][r]);
     if constexpr (SPLIT) {
       if (edge) {
         const int first = here(lane / (DV / 16));
@@ -239,7 +253,7 @@ struct Tree {
             x[i][u][r] = (int)(key >= lo) & (int)(key < hi) & (int)(kb + key > low[i]) ? x[i][u][r] : NEG;
           }
       }
-      softmax<NU, false>(i, x[i], inv, low_values);
+      softmax<NU, false>(i, x[i], inv, most);
       if constexpr (SPLIT) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) pq[i][u] = (f16x4){(_Float16)x[i][u][0], (_Float16)x[i][u][1], (_Float16)x[i][u][2], (_Float16)x[i][u][3]};
@@ -397,13 +411,12 @@ struct Tree {
         inv[u] = *(const f32x4*)&exps[32 + 16 * u + 4 * l4];
       }
     }
-    bool low_values = false;
+    float most = 0.f;
     if constexpr (CODES) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) low_values |= inv[u][r] > pow2(-LOWEST);
-      low_values = __any(low_values);
+        for (int r = 0; r < 4; ++r) most = fmaxf(most, inv[u][r]);
     }
     quad_t pq[NR][2][NOPND];
 #pragma unroll
@@ -419,7 +432,7 @@ struct Tree {
 #pragma unroll
           for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, key + 16 * u + r) ? x[i][u][r] : NEG;
       }
-      softmax<2, !CODES>(i, x[i], inv, low_values);
+      softmax<2, !CODES>(i, x[i], inv, most);
 #pragma unroll
       for (int u = 0; u < 2; ++u) split_quad(x[i][u], pq[i][u]);
     }

@@ -152,8 +152,9 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
   clear();
   const float inv_scale = 1.0f / p.scale;
 
-  // x: scores (with e / scale), unseen ones NEG -> weights; inv: 2^-e (one: there are none); low: some exponent is below LOWEST
-  auto softmax = [&](int i, auto& x, const auto& inv, auto one, bool low) {
+  Loudness loud;
+  // x: scores (with e / scale), unseen ones NEG -> weights; inv: 2^-e (one: there are none), mine: of the key whose number this lane has
+  auto softmax = [&](int i, auto& x, const auto& inv, auto one, float mine) {
     constexpr int U = sizeof(x) / sizeof(f32x4);
     float t = NEG;
 #pragma unroll
@@ -162,8 +163,15 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       for (int r = 0; r < 4; ++r) t = fmaxf(t, x[u][r]);
     t = rows_max(t);
     t = t <= NEG ? NEG : t * p.scale;
+    bool low = !one.value && loud.quiet(mine);
     const bool grows = t > m_run[i] + (low ? 0.f : LAZY);      // (the first key's always; a NaN never)
+    const bool some = __any(grows);
     const float m_new = grows ? t : m_run[i], m_sub = (m_new <= NEG ? 0.f : m_new) - W::SHIFT;
+    if constexpr (!one.value)
+      if (some) {
+        loud.set(-rows_max(lanes_max<16>(-mine)));
+        low = loud.quiet(mine);
+      }
     float own = 0.f, sum = 0.f;
     if (!one.value && low) {
 #pragma unroll
@@ -182,7 +190,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
         if constexpr (one.value) sum += x[u][r];
         else sum = __builtin_fmaf(x[u][r], inv[u][r], sum);
       }
-    if (__any(grows)) {
+    if (some) {
       const float root = root_of(m_run[i], m_new);
       l_run[i] = l_run[i] * root * root;
 #pragma unroll
@@ -210,8 +218,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
         }
     }
   };
-  // A tile of 32 keys and values in elements: products, weights, products; ev, inv: e / scale and 2^-e of a codes' kernel's drafted values, as those of codes
-  auto elem_products = [&](const uint8_t* kt, const uint8_t* vt, const frag_t (&q)[NR][DK / 32], bool edge, bool bad, const f32x4 (&ev)[2], const f32x4 (&inv)[2], bool low_values, int lo,
+  // A tile of 32 keys and values in elements: products, weights, products; ev, inv, mine: of a codes' kernel's drafted values, as those of codes
+  auto elem_products = [&](const uint8_t* kt, const uint8_t* vt, const frag_t (&q)[NR][DK / 32], bool edge, bool bad, const f32x4 (&ev)[2], const f32x4 (&inv)[2], float mine, int lo,
                            int hi, auto seen, auto value) {
     f32x4 x[NR][2];
 #pragma unroll
@@ -232,8 +240,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, key + 16 * u + r) ? x[i][u][r] : NEG;
       }
-      if constexpr (CODES) softmax(i, x[i], inv, No(), low_values);
-      else softmax(i, x[i], inv, Yes(), false);
+      if constexpr (CODES) softmax(i, x[i], inv, No(), mine);
+      else softmax(i, x[i], inv, Yes(), mine);
 #pragma unroll
       for (int u = 0; u < 2; ++u) split_quad(x[i][u], pq[i][u]);
     }
@@ -297,7 +305,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       if (live) {
         const elem_t* vb = (const elem_t*)p.vc + at * DV;
         const f32x4 none[2] = {};
-        elem_products(kt, vt, qf, edge, bad, none, none, false, lo, min(hi, KT), seen, [&](int j, int d) { return (float)vb[j * DV + d]; });
+        elem_products(kt, vt, qf, edge, bad, none, none, 0.f, lo, min(hi, KT), seen, [&](int j, int d) { return (float)vb[j * DV + d]; });
       }
     } else {
       uint8_t* exps = vt + W::VBYTES;
@@ -318,21 +326,18 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
         bad = shared[2] != 0;
       }
       if (live) {
-        f32x4* mine = (f32x4*)own;      // e / scale of 64 keys, then 2^-e
-        bool low_values;
-        {
-          const uint32_t b = exps[64 + lane];
-          low_values = __any((int)b < LOWEST + 127);
-          wave_sync();
-          ((float*)own)[lane] = ((float)b - 127.f) * inv_scale;
-          ((float*)own)[64 + lane] = __uint_as_float((254 - b) << 23);
-          wave_sync();
-        }
+        f32x4* both = (f32x4*)own;      // e / scale of 64 keys, then 2^-e
+        const uint32_t byte = exps[64 + lane];
+        const float mine = __uint_as_float((254 - byte) << 23);
+        wave_sync();
+        ((float*)own)[lane] = ((float)byte - 127.f) * inv_scale;
+        ((float*)own)[64 + lane] = mine;
+        wave_sync();
         f32x4 x[NR][NU], inv[NU];
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-          const f32x4 ev = mine[4 * u + l4];
-          inv[u] = mine[16 + 4 * u + l4];
+          const f32x4 ev = both[4 * u + l4];
+          inv[u] = both[16 + 4 * u + l4];
           const float scale = scale_of(exps[16 * u + l15]);
 #pragma unroll
           for (int j = 0; j < DK / 64; ++j) {
@@ -367,7 +372,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
 #pragma unroll
               for (int r = 0; r < 4; ++r) x[i][u][r] = seen(i, key + 16 * u + r) ? x[i][u][r] : NEG;
           }
-          softmax(i, x[i], inv, No(), low_values);
+          softmax(i, x[i], inv, No(), mine);
 #pragma unroll
           for (int u = 0; u < NU; ++u) pq[i][u] = (f16x4){(_Float16)x[i][u][0], (_Float16)x[i][u][1], (_Float16)x[i][u][2], (_Float16)x[i][u][3]};
         }
@@ -473,17 +478,17 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_wide_kernel(TreeArgs p) {
       for (int i = 0; i < NR; ++i)
         bits[i] = row_ok(i) && (j0 >> 6) < p.words ? (uint32_t)(p.mask[(int64_t)token_of(i) * p.words + (j0 >> 6)] >> (j0 & 63)) : 0u;
       f32x4 ev[2] = {}, inv[2] = {};
-      bool low_values = false;
+      float mine = 0.f;
       if constexpr (CODES) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           ev[u] = *(const f32x4*)&exps[16 * u + 4 * l4];
           inv[u] = *(const f32x4*)&exps[64 + 16 * u + 4 * l4];
         }
-        low_values = __any(exps[64 + (lane & 31)] > pow2(-LOWEST));
+        mine = exps[64 + (lane & 31)];
       }
       const elem_t* vb = p.v + row0 * p.ldv + (int64_t)s.g * DV;
-      elem_products(kt, vt, q, true, bad, ev, inv, low_values, 0, rows,
+      elem_products(kt, vt, q, true, bad, ev, inv, mine, 0, rows,
                     [&](int i, int key) {
                       return (bool)((int)(key < rows) & (int)(bits[i] >> key & 1) & (int)(p.pos[min((int)row0 + key, s.f0 + s.drafted - 1)] > low[i]));
                     },

@@ -160,3 +160,22 @@ def test_a_drafted_value_of_every_size():
         _check(c, c.run())
         c.length.zero_()
         _check(c, c.run())
+
+
+@pytest.mark.parametrize("low,high", [(-40, 100), (-60, 60), (-60, 115), (-100, 10), (0, 115), (-99, 115)])
+@pytest.mark.parametrize("first", ["quiet", "loud", "mixed"])
+@pytest.mark.parametrize("draft", [1, 20, 64])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_quiet_values_beside_loud_ones(dtype, draft, first, low, high):
+    """Rows under 2^low and 2^high: the quiet ones take their part of the sum, and keep their results where a window hides the loud"""
+    for context in (300, 3000):
+        c = Case(dtype, True, 64, 64, 4, 2, [(context, draft), (context // 2, draft)], kind="chain", seed=draft + high)
+        for b, n in enumerate(c.length.tolist()):
+            loud = torch.arange(n, device=dev()) % 3 == 0
+            loud = loud if first == "mixed" else torch.arange(n, device=dev()) < n // 2 if first == "loud" else torch.arange(n, device=dev()) >= n // 2
+            for page in range(-(-n // PAGE)):
+                at = loud[page * PAGE:(page + 1) * PAGE]
+                c.cache[3][int(c.bt[b, page]), :, :at.numel()] = torch.where(at, 127 + high, 127 + low).to(torch.uint8)
+        _check(c, c.run())
+        if first == "loud":
+            _check(c, c.run(window=context // 3), window=context // 3)
