@@ -35,6 +35,8 @@ __device__ __forceinline__ int bound_of(const TreeArgs& p, int pos) { return p.w
 // A row's weights are relative to a maximum that is followed only when it has grown by so much (in powers of two): what has been added up is rescaled in a
 // few tiles, not in every second one
 constexpr float LAZY = 8.f;
+// The largest weight over elements is 2^(LAZY + ELEMS_SHIFT): a sum of 2^24 values near the largest of their type stays finite
+constexpr float ELEMS_SHIFT = -32.f;
 // A weight is 2^(s + e - m'), and a probability it times 2^-e, so that a weight may be too small for 32 bits whose probability is not: where a tile has exponents
 // SPREAD below that of the keys which have set the maximum, or below LOWEST (the sum of many probabilities, each 2^-e times a weight, could pass 32
 // bits), the weights' roots are multiplied with 2^-e one by one.  What is lost otherwise is below 2^-30 of the largest probability.

@@ -29,7 +29,7 @@ __device__ __forceinline__ float inverse_of(uint32_t w, int i) { return __uint_a
 template <int DK, int DV, int NR, bool CODES>
 struct Tree {
   static constexpr bool F16 = CODES && SPLIT;                     // weights of codes are one f16 operand
-  static constexpr float SHIFT = F16 ? 7.f : 0.f;                  // an f16 weight is at most 2^(LAZY + 7)
+  static constexpr float SHIFT = F16 ? 7.f : CODES ? 0.f : ELEMS_SHIFT;      // an f16 weight is at most 2^(LAZY + 7)
   static constexpr int CH = DK / 64, PF = 16 / FR, NKF = CH * PF, NVB = DV / 16;
   static constexpr int KT = CODES ? 64 : 32, NU = KT / 16;        // keys of a context tile
   static constexpr int STAGE = 64 * DV;                           // bytes of a wave's V tile: 64 rows of codes, 32 of bf16

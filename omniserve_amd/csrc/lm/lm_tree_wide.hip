@@ -39,7 +39,7 @@ struct Wide {
   static constexpr int KP = KBYTES / 1024, VP = VBYTES / 1024, EACH = (KP + VP + NW - 1) / NW, PIECES = EACH + (CODES ? 2 : 0);      // of a wave
   static constexpr int OWN = CODES ? 512 : 0;                                     // a wave's: keys' exponents
   static constexpr int LDS = NBUF * SLOT + NW * OWN + 64;
-  static constexpr float SHIFT = CODES ? 7.f : 0.f;                              // weights of codes are f16: at most 2^(LAZY + 7)
+  static constexpr float SHIFT = CODES ? 7.f : ELEMS_SHIFT;                      // weights of codes are f16: at most 2^(LAZY + 7)
   typedef Tile<2 * DV> VT;
   typedef Tile<2 * DK> KTile;
 };

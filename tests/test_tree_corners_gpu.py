@@ -179,3 +179,19 @@ def test_quiet_values_beside_loud_ones(dtype, draft, first, low, high):
         _check(c, c.run())
         if first == "loud":
             _check(c, c.run(window=context // 3), window=context // 3)
+
+
+@pytest.mark.parametrize("draft", DRAFTS)
+@pytest.mark.parametrize("codes", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_values_near_the_largest(dtype, codes, draft):
+    """An average of numbers near the type's largest is a number"""
+    big = 2.0 ** 126
+    for context in (0, 300, 3000):
+        c = Case(dtype, codes, 64, 64, 4, 2, [(context, draft), (context // 2, draft)], seed=draft)
+        if not codes:
+            c.cache[1].copy_((c.cache[1].float().clamp(-1, 1) + torch.sign(c.cache[1].float())) * 0.75 * big)
+        c.v = ((c.v.float().clamp(-1, 1) + 2) * 0.6 * big).to(dtype)
+        got = c.run()
+        assert bool(got.isfinite().all())
+        _check(c, got)
