@@ -11,7 +11,7 @@
 extern "C" {
 #endif
 
-#define LM_ABI_VERSION 6
+#define LM_ABI_VERSION 7
 #define LM_NORM_LAYER 0
 #define LM_NORM_RMS 1
 #define LM_EPI_ELEM 0
@@ -77,16 +77,16 @@ int lm_attn_decode(const void* qkv, int64_t ld, const void* v_first, int64_t ldv
 
 /* ---- rotary positions, and a cache of 8-bit floats ----
  * Both pairings: halves 0 turns (2 i, 2 i + 1), else (i, i + half); the first 2 * half dimensions of a head turn, the others stay.
- * freq: f64, angle = position * freq[i] in 64 bits; cosine and sine times factor.  pos < 0: an empty place, nothing is done with its row. */
+ * freq: f64, angle = position * freq[i] in 64 bits; cosine and sine times factor, in 64 bits too.  pos < 0: an empty place, nothing is done with its row. */
 /* heads of dk at column 0 of every row of x -> the same columns of o: x itself (in place), or memory that does not overlap it. */
-int lm_rope(const void* x, int64_t ldx, void* o, int64_t ldo, const double* freq, int half, const int* pos, int halves, float factor,
+int lm_rope(const void* x, int64_t ldx, void* o, int64_t ldo, const double* freq, int half, const int* pos, int halves, double factor,
             int tokens, int heads, int dk, void* stream);
 /* Pools kc [pages][G][64][dk], vc [pages][G][64][dv] of e4m3 codes, ke, ve [pages][G][64]: value = code * 2^(byte - 127), the power (from
  * 2^-100) the least that brings the row's largest finite magnitude to 448; NaN and infinities become NaN.
  * Rows of x: q [H][dk] k [G][dk] v [G][dv].  half > 0: keys are turned (64 bits, rounded once) and, with q, the queries into q (row stride
  * ldq; x's own place or memory that does not overlap it).  half 0: keys as they are.  Token i is row i of x, or rows[i] (then q is null; rows
  * outside 0 .. x_rows - 1 are none); slot[i] = page * 64 + offset, outside the pools: not stored.  No two tokens of a call have the same slot. */
-int lm_kv_store(const void* x, int64_t ldx, int x_rows, const int* rows, const double* freq, int half, const int* pos, int halves, float factor,
+int lm_kv_store(const void* x, int64_t ldx, int x_rows, const int* rows, const double* freq, int half, const int* pos, int halves, double factor,
                 void* q, int64_t ldq, const int* slot, uint8_t* kc, uint8_t* vc, uint8_t* ke, uint8_t* ve, int64_t pages, int tokens, int H,
                 int G, int dk, int dv, void* stream);
 /* k [tokens][G][dk], v [tokens][G][dv] of the places slot[i]; zeros for a slot outside the pools. */

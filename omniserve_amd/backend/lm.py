@@ -14,13 +14,13 @@ import torch
 from .. import _lib
 
 _c = ctypes
-_vp, _i, _i64, _f = _c.c_void_p, _c.c_int, _c.c_int64, _c.c_float
+_vp, _i, _i64, _f, _d = _c.c_void_p, _c.c_int, _c.c_int64, _c.c_float, _c.c_double
 
 ELEM = {torch.bfloat16: "bf16", torch.float32: "f32"}
 NORM = {"layer": 0, "rms": 1}
 ACT = {None: 0, "silu": 1, "gelu_tanh": 2, "sigmoid": 3}
 EPI_ELEM, EPI_F32, EPI_GLU, EPI_GATE = 0, 1, 2, 3
-ABI = 6
+ABI = 7
 ATTN_ROWS = 128          # query rows of one prefill tile
 PAGE = 64                # tokens per cache page
 ROWS_MAX = 64            # up to here a step's products stream the weights
@@ -46,8 +46,8 @@ PROTOTYPES = {
     "lm_attn_prefill_rows": (_i, [_i, _i, _i, _i]),
     "lm_attn_decode": (_i, [_vp, _i64, _vp, _i64, _f, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i64, _vp, _i64, _vp, _i, _f, _i, _i, _i,
                             _i, _i, _i, _vp]),
-    "lm_rope": (_i, [_vp, _i64, _vp, _i64, _vp, _i, _vp, _i, _f, _i, _i, _i, _vp]),
-    "lm_kv_store": (_i, [_vp, _i64, _i, _vp, _vp, _i, _vp, _i, _f, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
+    "lm_rope": (_i, [_vp, _i64, _vp, _i64, _vp, _i, _vp, _i, _d, _i, _i, _i, _vp]),
+    "lm_kv_store": (_i, [_vp, _i64, _i, _vp, _vp, _i, _vp, _i, _d, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
     "lm_kv_load": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i, _i, _i, _i, _vp]),
     "lm_tree_attn_scratch": (_i64, [_i] * 8),
     "lm_tree_attn": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _i64, _vp, _f,

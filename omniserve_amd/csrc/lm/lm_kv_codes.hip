@@ -16,7 +16,7 @@ struct Turn {
   const double* freq;      // per pair; half = 0: nothing turns
   const int* pos;          // < 0: an empty place
   int half, halves;        // pairs (i, i + half) instead of (2 i, 2 i + 1)
-  float factor;
+  double factor;
 };
 
 struct RopeArgs {
@@ -316,7 +316,7 @@ static RopeArgs rope_args(const void* x, int64_t ldx, void* o, int64_t ldo, cons
 
 using namespace lm;
 
-extern "C" int lm_rope(const void* x, int64_t ldx, void* o, int64_t ldo, const double* freq, int half, const int* pos, int halves, float factor,
+extern "C" int lm_rope(const void* x, int64_t ldx, void* o, int64_t ldo, const double* freq, int half, const int* pos, int halves, double factor,
                        int tokens, int heads, int dk, void* stream) {
   if (tokens < 0 || heads <= 0 || heads > MOST_HEADS || dk <= 0 || half < 1 || !good_turn(freq, half, pos, dk) || (tokens && (!x || !o))) return LM_EINVAL;
   if (tokens == 0) return LM_OK;
@@ -331,7 +331,7 @@ extern "C" int lm_rope(const void* x, int64_t ldx, void* o, int64_t ldo, const d
 
 static bool code_size(int d) { return d == 64 || d == 128 || d == 256; }
 
-extern "C" int lm_kv_store(const void* x, int64_t ldx, int x_rows, const int* rows, const double* freq, int half, const int* pos, int halves, float factor, void* q,
+extern "C" int lm_kv_store(const void* x, int64_t ldx, int x_rows, const int* rows, const double* freq, int half, const int* pos, int halves, double factor, void* q,
                            int64_t ldq, const int* slot, uint8_t* kc, uint8_t* vc, uint8_t* ke, uint8_t* ve, int64_t pages, int tokens, int H, int G, int dk,
                            int dv, void* stream) {
   if (tokens < 0 || H < 0 || G <= 0 || H + G > MOST_HEADS || !code_size(dk) || !code_size(dv) || !good_turn(freq, half, pos, dk) || pages < 0 || pages * PAGE > INT32_MAX ||

@@ -121,7 +121,7 @@ class Ops {
     one_device(x, {}, {opt(freq), opt(pos), opt(out)});
     const c10::DeviceGuard guard(x.device());
     const T o = out ? *out : torch::empty({n, w}, x.options());
-    done(rope_(x.data_ptr(), step(x), o.data_ptr(), step(o), t.freq, t.half, t.pos, t.halves, (float)factor, narrow(n), (int)heads, (int)dk, stream(x)), "lm_rope");
+    done(rope_(x.data_ptr(), step(x), o.data_ptr(), step(o), t.freq, t.half, t.pos, t.halves, factor, narrow(n), (int)heads, (int)dk, stream(x)), "lm_rope");
     return o;
   }
 
@@ -138,7 +138,7 @@ class Ops {
     if (picked) index(*picked, n, "rows");
     one_device(x, cache, {&slot, opt(freq), opt(pos), opt(q_out), opt(picked)});
     const c10::DeviceGuard guard(x.device());
-    done(store_(x.data_ptr(), step(x), narrow(x.size(0)), (const int*)ptr(picked), t.freq, t.half, t.pos, t.halves, (float)factor, ptr(q_out), q_out ? step(*q_out) : 0,
+    done(store_(x.data_ptr(), step(x), narrow(x.size(0)), (const int*)ptr(picked), t.freq, t.half, t.pos, t.halves, factor, ptr(q_out), q_out ? step(*q_out) : 0,
                 slot.data_ptr<int>(), cache[0].data_ptr<uint8_t>(), cache[1].data_ptr<uint8_t>(), cache[2].data_ptr<uint8_t>(), cache[3].data_ptr<uint8_t>(), s.pages, narrow(n),
                 (int)heads, narrow(s.G), (int)s.dk, (int)s.dv, stream(x)),
          "lm_kv_store");
