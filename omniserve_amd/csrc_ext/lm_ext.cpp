@@ -1,7 +1,8 @@
 // Checks and marshalling of the engine's operators that a program calls for single tokens (include/omniserve_lm.h: rotary positions, the quantised cache,
 // drafted tokens): a call's dozen tensors are looked over, its result and scratch allocated and the entry point called in 3 - 5 us, where the same in
 // Python takes 12 - 40 (more than the kernels of such a call).  No kernel lives here; the entry points are those of the library that the Python side has
-// loaded, handed over by address, one Ops per element type.  Refusals are ValueErrors, before anything is enqueued; the library's own are RuntimeErrors.
+// loaded, handed over by address, one Ops per element type.  A call that does not fit is a ValueError, before anything is enqueued, the library's own refusals
+// among them; a launch that fails is a RuntimeError.
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -24,6 +25,7 @@ typedef std::vector<T> Pools;
 
 constexpr int64_t PAGE = 64;
 constexpr int NO_WINDOW = INT32_MAX;
+constexpr int64_t MOST_HEADS = 4096, MOST_ROWS = 1 << 24;      // of a row; drafted tokens times heads
 
 template <typename... What>
 inline void need(bool ok, const What&... what) {
@@ -32,7 +34,8 @@ inline void need(bool ok, const What&... what) {
 
 inline void done(int rc, const char* name) {
   if (rc == 0) return;
-  throw std::runtime_error(std::string(name) + " failed: " + (rc == -22 ? "invalid argument" : rc == -5 ? "kernel launch failed" : "error") + " (" + std::to_string(rc) + ")");
+  if (rc == -22) throw py::value_error(std::string(name) + ": sizes, strides or addresses that it does not take");
+  throw std::runtime_error(std::string(name) + " failed: " + (rc == -5 ? "kernel launch failed" : "error") + " (" + std::to_string(rc) + ")");
 }
 
 // from row to row (a single row's stride may be anything)
@@ -67,6 +70,11 @@ class Ops {
   void rows(const T& t, int64_t width, int64_t n, const char* name) const {
     need(t.dim() == 2 && t.size(1) >= width && t.scalar_type() == elem && (t.stride(1) == 1 || t.size(1) == 1), name, ": rows of ", width, " or more ", elem);
     need(n < 0 || t.size(0) == n, name, ": ", n, " rows");
+  }
+  // ... that a call writes: no two of them share memory
+  void results(const T& t, int64_t width, int64_t n, const char* name) const {
+    rows(t, width, n, name);
+    need(t.size(0) <= 1 || t.stride(0) >= width, name, ": rows that do not overlap");
   }
 
   static Turn turn(const OptT& freq, const OptT& pos, int64_t n, int64_t dk, const std::string& pairing) {
@@ -111,13 +119,13 @@ class Ops {
         scratch_((decltype(scratch_))scratch), tree_((decltype(tree_))tree) {}
 
   T rope(const T& x, const OptT& freq, const OptT& pos, int64_t heads, int64_t dk, const std::string& pairing, double factor, const OptT& out) const {
-    need(heads > 0 && dk > 0 && heads <= INT32_MAX && dk <= INT32_MAX, "heads of at least one dimension");
+    need(heads > 0 && heads <= MOST_HEADS && dk > 0 && dk <= INT32_MAX, "heads: 1 to ", MOST_HEADS, ", of at least one dimension");
     const int64_t w = heads * dk;
     rows(x, w, -1, "x");
     const int64_t n = x.size(0);
     const Turn t = turn(freq, pos, n, dk, pairing);
     need(t.half > 0, "freq and pos say how rope turns");
-    if (out) rows(*out, w, n, "out");
+    if (out) results(*out, w, n, "out");
     one_device(x, {}, {opt(freq), opt(pos), opt(out)});
     const c10::DeviceGuard guard(x.device());
     const T o = out ? *out : torch::empty({n, w}, x.options());
@@ -128,13 +136,14 @@ class Ops {
   void kv_store(const T& x, const Pools& cache, const T& slot, int64_t heads, const OptT& freq, const OptT& pos, const std::string& pairing, double factor, const OptT& q_out,
                 const OptT& picked) const {
     const Sizes s = pools(cache, true);
-    need(heads >= 0 && heads <= INT32_MAX, "heads: none or more");
+    need(heads >= 0 && heads + s.G <= MOST_HEADS, "heads: none or more, ", MOST_HEADS, " at most with the kv heads");
+    need((uintptr_t)cache[0].data_ptr() % 8 == 0 && (uintptr_t)cache[1].data_ptr() % 8 == 0, "cache: pools at 8 bytes");
     rows(x, (heads + s.G) * s.dk + s.G * s.dv, -1, "x");
     const int64_t n = picked ? slot.size(0) : x.size(0);
     index(slot, n, "slot");
     const Turn t = turn(freq, pos, n, s.dk, pairing);
     need(!q_out || (!picked && heads > 0 && t.half > 0), "queries are turned of all rows in order");
-    if (q_out) rows(*q_out, heads * s.dk, n, "q_out");
+    if (q_out) results(*q_out, heads * s.dk, n, "q_out");
     if (picked) index(*picked, n, "rows");
     one_device(x, cache, {&slot, opt(freq), opt(pos), opt(q_out), opt(picked)});
     const c10::DeviceGuard guard(x.device());
@@ -149,9 +158,11 @@ class Ops {
     need(slot.dim() == 1, "slot: a vector");
     const int64_t n = slot.size(0);
     index(slot, n, "slot");
+    need(s.G <= MOST_HEADS, "kv heads: ", MOST_HEADS, " at most");
+    need((uintptr_t)cache[0].data_ptr() % 16 == 0 && (uintptr_t)cache[1].data_ptr() % 16 == 0, "cache: pools at 16 bytes");
     if (out) {
-      rows(std::get<0>(*out), s.G * s.dk, n, "out");
-      rows(std::get<1>(*out), s.G * s.dv, n, "out");
+      results(std::get<0>(*out), s.G * s.dk, n, "out");
+      results(std::get<1>(*out), s.G * s.dv, n, "out");
       need(at16(std::get<0>(*out)) && at16(std::get<1>(*out)), "out: rows at 16 bytes");
       one_device(slot, {}, {&std::get<0>(*out), &std::get<1>(*out)});
     }
@@ -186,11 +197,13 @@ class Ops {
     index(pos, n, "pos");
     index(length, B, "length");
     need(bt.scalar_type() == torch::kInt32 && bt.dim() == 2 && bt.size(0) == B && (bt.stride(1) == 1 || bt.size(1) <= 1), "bt: int32 [sequences, pages]");
+    need(B <= 1 || bt.stride(0) >= bt.size(1), "bt: rows that do not overlap");
     need(bt.size(1) == 0 || s.pages > 0, "a block table needs pages");
+    need(max_draft * H <= MOST_ROWS, "max_draft: ", MOST_ROWS, " rows of tokens times heads at most");
     need(scale >= 0x1p-60 && scale <= 0x1p60 && (!window || *window > 0), "scale: 2^-60 to 2^60; window: positive");
     need(max_context >= 0, "max_context is a number of keys");
     if (out) {
-      rows(*out, H * s.dv, n, "out");
+      results(*out, H * s.dv, n, "out");
       need((uintptr_t)out->data_ptr() % (4 * out->element_size()) == 0 && step(*out) % 4 == 0, "out: rows at four elements");
     }
     one_device(q, cache, {&k, &v, &mask, &first, &pos, &bt, &length, opt(out)});
