@@ -195,3 +195,52 @@ def test_values_near_the_largest(dtype, codes, draft):
         got = c.run()
         assert bool(got.isfinite().all())
         _check(c, got)
+
+
+@pytest.mark.parametrize("draft", [1, 6, 13, 20, 64])
+@pytest.mark.parametrize("window", [1, 40, 64, 65, 130, 1000, 2500])
+@pytest.mark.parametrize("codes", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_windows_over_short_and_long_contexts(dtype, codes, window, draft):
+    """Few and many rows, segments in one piece and cut, whose first pages no row sees; a table of page numbers that are none in front of the windows"""
+    for kind in ("chain", "tree"):
+        c = Case(dtype, codes, 64, 64, 4, 2, [(3000, draft), (300, draft), (64, 1), (129, draft), (0, draft)], kind=kind, seed=window + draft)
+        _check(c, c.run(window=window), window)
+        want = c.run(window=window)
+        for b, n in enumerate(c.length.tolist()):
+            c.bt[b, :max(0, n + 1 - window) // PAGE] = -7
+        assert torch.equal(c.run(window=window), want)
+
+
+@pytest.mark.parametrize("draft", [1, 6, 13, 20, 64])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("codes", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_nothing_comes_out_of_places_that_no_row_sees(dtype, codes, bad, draft):
+    """Behind the end of the last page and in front of every window, keys, values and exponents of any bits"""
+    for window in (None, 120, 2000):
+        c = Case(dtype, codes, 128, 64, 4, 2, [(3000, draft), (100, draft), (300, draft), (64, draft)], seed=draft)
+        want = c.run(window=window)
+        for b, n in enumerate(c.length.tolist()):
+            for key in list(range(n, -(-n // PAGE) * PAGE)) + list(range(max(0, n + 1 - (window or n + 1)))):
+                page = int(c.bt[b, key // PAGE])
+                for i in (0, 1):
+                    c.cache[i][page, :, key % PAGE] = 0x7f if codes else bad
+                    if codes:
+                        c.cache[2 + i][page, :, key % PAGE] = 255 if bad > 0 else 254
+        got = c.run(window=window)
+        assert torch.equal(got, want) and bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("draft", [1, 6, 13, 20, 64, 150])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("codes", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_bad_values_that_some_rows_see(dtype, codes, bad, draft):
+    """A cached value that is not finite (of codes: NaN), seen by the rows whose windows reach it: in the first page of a window, in the last one, in between"""
+    for window in (90, 700):
+        for back in (0, 1, draft // 2, 64, window - draft // 2 - 1, window - 2):
+            c = Case(dtype, codes, 64, 64, 4, 2, [(3000, draft), (800, draft)], kind="chain", seed=window)
+            _spoil(c, 0, 2999 - back, bad)
+            _spoil(c, 1, 799 - back, bad, 17)
+            _check(c, c.run(window=window), window)
