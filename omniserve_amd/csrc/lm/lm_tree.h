@@ -47,15 +47,15 @@ constexpr int LOWEST = -63, SPREAD = 96;
 // finite is below 2^-124 after two times the least)
 __device__ __forceinline__ float root_of(float m, float m_new) { return fmaxf(__builtin_amdgcn_exp2f(0.5f * (m - m_new)), 0x1p-126f); }
 
-// Which tiles those are, of one wave.  Exponents are looked at as 2^-e.
+// Which tiles those are, of one wave.  Exponents are looked at as the bits of 2^-e, in scalar registers.
 struct Loudness {
-  float loudest, limit;      // of the keys that have set a maximum; of the tiles that go without roots
-  __device__ __forceinline__ Loudness() : loudest(__builtin_inff()), limit(pow2(-LOWEST)) {}
-  __device__ __forceinline__ bool quiet(float most) const { return __any(most > limit); }      // most: the largest of this lane's
+  static constexpr uint32_t FROM = (uint32_t)(127 - LOWEST) << 23;
+  uint32_t loudest = ~0u, limit = FROM;      // of the keys that have set a maximum; of the tiles that go without roots
+  __device__ __forceinline__ bool quiet(float most) const { return __any(__float_as_uint(most) > limit); }      // most: the largest of this lane's
   // a tile sets a row's maximum; least: the smallest of all its keys'
   __device__ __forceinline__ void set(float least) {
-    loudest = fminf(loudest, least);
-    limit = fminf(pow2(-LOWEST), loudest * pow2(SPREAD));
+    loudest = min(loudest, (uint32_t)__builtin_amdgcn_readfirstlane(__float_as_uint(least)));
+    limit = min(FROM, loudest + ((uint32_t)SPREAD << 23));
   }
 };
 
@@ -143,7 +143,7 @@ __device__ __forceinline__ uint32_t drop_nan_codes(uint32_t w, bool& bad) {
 // A segment is the keys of one (sequence, kv head, block of rows): its context tiles that any row sees and, behind them, tiles of 32 drafted tokens.
 // Where segments are few or of different lengths they are cut into equal pieces of at most run_length() tiles, a workgroup each.  The length follows from
 // the tiles of all of them, so that there are as many pieces as suit the chip whatever the sequences' lengths are (a fixed number of parts a sequence
-// leaves the short ones' places idle: 16 trees of 26 over 500 - 4000 keys 65 us, with pieces of one length 58).  A segment of one piece is written by it, others are joined by tree_merge_kernel.  The division depends on the
+// leaves the short ones' places idle: 16 trees of 26 over 500 - 4000 keys took 65 us where pieces of one length took 58, when the pieces themselves were slower than now).  A segment of one piece is written by it, others are joined by tree_merge_kernel.  The division depends on the
 // lengths alone.
 
 struct Segments {            // of one sequence

@@ -8,15 +8,15 @@
 // cache holds codes) in turn, so that a key's codes are fetched and decoded once for all rows, and meet in LDS.  More than 32 rows (16 of heads of
 // 256) go to lm_tree_wide.hip.
 //
-// Bound by the cache's bytes where there are enough of them: 61 tokens over 300 - 4000 keys of 8 heads of 128 72 us, 281 MB at 3.9 TB/s;
-// one over 1501 keys 15 us, 4 of them the joining launch.  (Three waves a SIMD spill: 73 -> 114 us.  Eight waves a workgroup: 87.)
+// Bound by the cache's bytes where there are enough of them: 61 tokens over 300 - 4000 keys of 8 heads of 128 71 us a call, 281 MB at 4.0 TB/s;
+// one over 1501 keys 14.2 us, 4 of them the joining launch.  (Three waves a SIMD spill: 73 -> 114 us.  Eight waves a workgroup: 87.)
 //
 // Codes (lm_kv_codes.h).  A key's power of two scales its operand in the conversion.  A value's, 2^e, joins the softmax: with weights
 // w_j = 2^(s_j + e_j - m'), m' the running maximum of s_j + e_j, the outputs are sum w_j code_j and the sum of the probabilities is
 // sum w_j 2^(-e_j).  So w_j is at most 2^LAZY and is ONE f16 operand (11 bits, times 2^7 so that small ones stay normal) beside codes that f16
 // holds exactly; bf16 values need two bf16 operands for theirs (16 bits).  A drafted token's values are divided by such a power of two of their own first, so
-// that nothing depends on the size of values that a row does not see.  A tile with rows of very small values, or none but zeros (2^-100), beside which the others' maximum leaves
-// such a weight nothing, multiplies its roots with 2^(-e) one by one: its rows count in the sum as all others do.
+// that nothing depends on the size of values that a row does not see.  A tile with rows of values so much smaller than the others' (or none but zeros, 2^-100) that the maximum leaves
+// such a weight nothing multiplies its roots with 2^(-e) one by one (Loudness): its rows count in the sum as all others do.
 #include "lm_tree.h"
 #include "omniserve_lm.h"
 
@@ -189,7 +189,6 @@ struct Tree {
         }
     }
     const uint8_t* vp = p.vc + c.at * DV;
-    f32x4 ev[NU], inv[NU];
     bool bad = false;
     if (edge) {
       const int k4 = here(4 * l4);
@@ -204,15 +203,6 @@ struct Tree {
         c.vx[u] = w;
       }
     }
-#pragma unroll
-    for (int u = 0; u < NU; ++u)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) { ev[u][r] = exponent_of(c.vx[u], r); inv[u][r] = inverse_of(c.vx[u], r); }
-    float most = inv[0][0];
-#pragma unroll
-    for (int u = 0; u < NU; ++u)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) most = fmaxf(most, inv[u][r]);
     if constexpr (SPLIT) {
       if (edge) {
         const int first = here(lane / (DV / 16));
@@ -234,8 +224,21 @@ struct Tree {
       }
     }
     const int64_t page_at = c.at;
+    uint32_t vx[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) vx[u] = c.vx[u];
     next();
     if constexpr (SPLIT) wave_sync();
+    f32x4 ev[NU], inv[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) { ev[u][r] = exponent_of(vx[u], r); inv[u][r] = inverse_of(vx[u], r); }
+    float most = inv[0][0];
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) most = fmaxf(most, inv[u][r]);
     f16x4 pq[NR][NU];
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
@@ -344,46 +347,44 @@ struct Tree {
     const int64_t ldv = c.ldv;
     f32x4 ev[2], inv[2];      // of this lane's keys, as those of codes
     if constexpr (SPLIT) {
-      float of[CODES ? DV / 16 : 1];      // exponents of the rows that this lane has a part of
+      __builtin_amdgcn_wave_barrier();       // the previous tile has been read
       if (edge) {
 #pragma unroll
         for (int i = 0; i < DV / 16; ++i) {
+          const int at = 64 * i + lane, row = at / (DV / 8);
+          int e = 0;
           if (64 * i / (DV / 8) >= hi) {      // (a step without drafts has one row)
             c.v[i] = frag_t{};
-            if constexpr (CODES) of[i] = 0.f;
-            continue;
-          }
-          const int row = (64 * i + lane) / (DV / 8);
-          float top = 0.f;
+          } else {
+            float top = 0.f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            float y = row >= lo && row < hi ? (float)c.v[i][k] : 0.f;
-            const bool fine = fabsf(y) < __builtin_inff();
-            bad |= !fine;
-            y = fine ? y : 0.f;
-            top = fmaxf(top, fabsf(y));
-            c.v[i][k] = (elem_t)y;
-          }
-          if constexpr (CODES) {
-            const int e = row >= lo && row < hi ? row_exponent(lanes_max<DV / 8>(top)) : 0;
-            const float f = pow2(-e);
-            of[i] = (float)e;
+            for (int k = 0; k < 8; ++k) {
+              float y = row >= lo && row < hi ? (float)c.v[i][k] : 0.f;
+              const bool fine = fabsf(y) < __builtin_inff();
+              bad |= !fine;
+              y = fine ? y : 0.f;
+              top = fmaxf(top, fabsf(y));
+              c.v[i][k] = (elem_t)y;
+            }
+            if constexpr (CODES) {
+              e = row >= lo && row < hi ? row_exponent(lanes_max<DV / 8>(top)) : 0;
+              const float f = pow2(-e);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) c.v[i][k] = (elem_t)((float)c.v[i][k] * f);
+              for (int k = 0; k < 8; ++k) c.v[i][k] = (elem_t)((float)c.v[i][k] * f);
+            }
           }
+          if constexpr (CODES)
+            if (at % VT::NS == 0) {
+              exps[row] = (float)e;
+              exps[32 + row] = pow2(-e);
+            }
         }
         bad = __any(bad);
       }
-      __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int i = 0; i < DV / 16; ++i) {
         const int at = 64 * i + lane;
         *(frag_t*)(stage + VT::slot(at / VT::NS, at % VT::NS)) = c.v[i];
-        if constexpr (CODES)
-          if (at % VT::NS == 0) {
-            exps[at / VT::NS] = of[i];
-            exps[32 + at / VT::NS] = pow2(-(int)of[i]);
-          }
       }
     } else if constexpr (CODES) {
 #pragma unroll
@@ -715,9 +716,10 @@ struct Plan {
   int64_t run, blocks, workgroups, target, scratch;
 };
 // Cut where the segments are fewer than four rounds of workgroups and the longest has more tiles than joining is worth: 20 of the narrow kernel, 8 of the wide
-// one (one token, 1501 keys of 8 heads in one piece each 17.2 us, in pieces of 4 tiles 14.9; 16 of 1024 keys 17.1 and 20.2; a tree of 26, 500 keys, in one
-// piece 29.0, in pieces of 3 tiles 25.6).  Into as many pieces as workgroups fit the chip, or twice as many where the segments alone are half of that (61 tokens of
-// 300 - 4000 keys: 76 us and 73; the wide kernel, whose pieces have more sums to write, not: 4 trees of 64 over 32768 keys 227 instead of 183).
+// one (one token, 1501 keys of 8 heads in one piece each 14.9 us, in pieces of 4 tiles 14.4; 16 of 1024 keys 13.6 and 19.3; a tree of 26, 500 keys, in one
+// piece 25.7, in pieces of 3 tiles 20.8).  Into as many pieces as workgroups fit the chip, or twice as many where the segments alone are half of that (61 tokens of
+// 300 - 4000 keys: 74 us and 70; the wide kernel, whose pieces have more sums to write, not: 4 trees of 64 over 32768 keys 240 instead of 212, a tree of 26 for each
+// of 16 sequences 58 instead of 47).
 static Plan plan_of(int B, int max_draft, int max_context, int H, int G, int dk, int dv, bool codes) {
   Plan q{};
   const int rows = max_draft * (H / G), kt = codes ? 64 : 32;
