@@ -81,8 +81,8 @@ int lm_attn_decode(const void* qkv, int64_t ld, const void* v_first, int64_t ldv
 /* heads of dk at column 0 of every row of x -> the same columns of o: x itself (in place), or memory that does not overlap it. */
 int lm_rope(const void* x, int64_t ldx, void* o, int64_t ldo, const double* freq, int half, const int* pos, int halves, double factor,
             int tokens, int heads, int dk, void* stream);
-/* Pools kc [pages][G][64][dk], vc [pages][G][64][dv] of e4m3 codes, ke, ve [pages][G][64]: value = code * 2^(byte - 127), the power (from
- * 2^-100) the least that brings the row's largest finite magnitude to 448; NaN and infinities become NaN.
+/* Pools kc [pages][G][64][dk], vc [pages][G][64][dv] of e4m3 codes, ke, ve [pages][G][64]: value = code * 2^(byte - 127), the power the least
+ * from 2^-100 to 2^120 (bytes 27 to 247; what a place of another byte holds is unspecified) that brings the row's largest finite magnitude to 448; NaN and infinities become NaN.
  * Rows of x: q [H][dk] k [G][dk] v [G][dv].  half > 0: keys are turned (64 bits, rounded once) and, with q, the queries into q (row stride
  * ldq; x's own place or memory that does not overlap it).  half 0: keys as they are.  Token i is row i of x, or rows[i] (then q is null; rows
  * outside 0 .. x_rows - 1 are none); slot[i] = page * 64 + offset, outside the pools: not stored.  No two tokens of a call have the same slot. */
@@ -94,7 +94,8 @@ int lm_kv_load(void* k, int64_t ldk, void* v, int64_t ldv, const uint8_t* kc, co
                int64_t pages, const int* slot, int tokens, int G, int dk, int dv, void* stream);
 /* Attention of drafted tokens: sequence b has tokens first[b] .. first[b + 1] - 1 of q [H][dk], k [G][dk], v [G][dv] (positions pos, turned
  * already; at most max_draft, further ones are left out) and length[b] keys in the pages bt[b].  A token sees the context, and drafted token j of its sequence
- * where bit j % 64 of mask[token][j / 64] is set, both only from position pos - window + 1 on.  It sees nothing: zeros.  Pools as above, or
+ * where bit j % 64 of mask[token][j / 64] is set, both only from position pos - window + 1 on.  It sees nothing: zeros.  Scores of -1e30 or
+ * less (q . k, or that times scale) may count as unseen.  Pools as above, or
  * (ke, ve null) of elem; pages outside 0 .. pages - 1 are not seen.  part: lm_tree_attn_scratch() f32 for these
  * sizes, by which the keys of few or unequal sequences are dealt out (null: a workgroup has all keys of its rows); max_context: bound of the
  * lengths, a hint.  window INT32_MAX: none. */

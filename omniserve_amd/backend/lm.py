@@ -96,7 +96,7 @@ def _ld(t):
 
 class KvCodes(NamedTuple):
     """A layer's quantised cache: e4m3 codes [pages, kv heads, 64, size] and their rows' exponents [pages, kv heads, 64], all uint8; value =
-    code * 2^(exponent - 127).  1 / 64 .. 1 / 256 more than a byte an element."""
+    code * 2^(exponent - 127), exponents from 27 (code_pools' own) to 247.  1 / 64 .. 1 / 256 more than a byte an element."""
     k: torch.Tensor
     v: torch.Tensor
     k_exp: torch.Tensor
@@ -211,7 +211,8 @@ class LmOps:
     def kv_store(self, x, cache, slot, heads, *, freq=None, pos=None, pairing="neighbours", factor=1.0, q_out=None, rows=None):
         """Keys and values of rows x (q [heads] k [kv heads] v [kv heads]) into a quantised cache (KvCodes) at slot = page * 64 + offset; a slot outside
         the pools is not stored, no two tokens have the same.  freq, pos: keys are turned first, and with q_out (x's own columns, or memory that does
-        not overlap x) the queries too.  rows: token i is row rows[i] of x (of drafted tokens, those that were kept)."""
+        not overlap x) the queries too.  rows: token i is row rows[i] of x (of drafted tokens, those that were kept: of unturned rows, with their freq and pos, the codes
+        are those of a prompt; rows that rope has turned are rounded a second time)."""
         self._x.kv_store(x, cache, slot, heads, freq, pos, pairing, factor, q_out, rows)
 
     def kv_load(self, cache, slot, out=None):
@@ -225,7 +226,8 @@ class LmOps:
         keys in the pages bt[b].  A token sees the cached keys and, of its sequence, the drafted ones whose bit is set in mask [tokens, words] (int64, tree_masks); with a
         window only those at positions above its pos - window.  Rows that see nothing are zero; rows of no sequence stay as they are (without out they are unspecified).  cache: KvCodes, or
         (keys, values) [pages, kv heads, 64, size] of elements.  max_context: a bound of the lengths, by which the work is divided (longer ones are
-        attended to as well).  scale: 2^-60 to 2^60.  out: memory of its own."""
+        attended to as well).  scale: 2^-60 to 2^60.  out: memory of its own.
+        Scores, their maximum and all sums are f32; of bf16 a softmax weight has 11 bits over codes and 16 over elements."""
         return self._x.tree_attn(q, k, v, mask, first, pos, cache, bt, length, scale, window, max_draft, max_context, out)
 
     def linear_prefill(self, x, o, state, seg_state, seg, seg_len, multi, log2_decay, heads, dk, dv, act):

@@ -1,8 +1,8 @@
 // Rotary positions of queries and keys, and the cache of 8-bit keys and values (lm_kv_codes.h): written with the rotation in the same
-// launch, read back as rows.  All three are bound by memory: 12001 tokens of 40 heads of 128, half of each turned, 38.5 us, of 64 heads over 8 turned and stored 109, 100000
-// tokens of 8 heads read back 124 (6.4, 4.3 and 4.9 TB/s read and written; a copy of 8 GB 4.8).
+// launch, read back as rows.  All three are bound by memory: kernels of 12001 tokens of 40 heads of 128, half of each turned, 38.7 us, of 64 heads over 8 turned and stored 109,
+// of 100000 tokens of 8 heads read back 125 (6.4, 4.3 and 4.9 TB/s read and written; a copy of 8 GB 4.8).
 //
-// Angles: position * frequency in 64 bits (a frequency of one and a position of a million leave 2^-4 of a turn's accuracy in 32), taken
+// Angles: position * frequency in 64 bits (32 hold an angle of a million radians to 2^-5 of one, a two-hundredth of a turn), taken
 // modulo a turn and through sincospi once per token and pair, by the workgroup, for all of its heads.
 //
 // A workgroup takes a few tokens, so that its threads have several 16-byte pieces each and the sines are formed by all of them; few

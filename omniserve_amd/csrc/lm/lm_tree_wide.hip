@@ -2,14 +2,14 @@
 // value tiles that DMA fills two tiles ahead.  See lm_tree_attn.hip for the formula; here a tile is 64 keys of codes, or 32 of elements.
 //
 // Bound by the vector units beside the matrix units (a softmax weight costs 4 vector instructions, one of them an exponential of four times the
-// length, and 256 operations of the matrix units), so that what a weight does not need is done elsewhere:
-//   a key is decoded with its power of two into bf16, which holds it exactly.  (Products of the codes themselves, at twice the rate and without the decoding, take 175 us
-//     where this takes 205, but the matrix units add products of 8-bit floats in fewer than 32 bits: a sum of 128 was off by up to 2^-12 of its largest product, of
-//     bf16 by 2^-21);
+// length, and 256 operations of the matrix units), and by the latency between them, so that what a weight does not need is done elsewhere:
+//   a key is decoded with its power of two into bf16, which holds it exactly.  (Products of the codes themselves, at twice the rate and without the decoding, made
+//     4 trees of 64 over 32768 keys 175 us where this takes 205, but the matrix units add products of 8-bit floats in fewer than 32 bits: a sum of 128 was off by
+//     up to 2^-12 of its largest product, of bf16 by 2^-21);
 //   a value's exponent (lm_tree_attn.hip) is the products' initial accumulator, e / scale;
 //   2^-e and e / scale are formed by one lane per key and read back from LDS.
-// 4 trees of 64 over 32768 keys, 32 heads over 8: 174 us, 0.77 PFLOP/s; matrix units busy 36 % of the time, vector units 56, no LDS conflicts
-// (workgroups of half the rows 188 for 183 us; staggered starts 173 for 176; the products at higher priority: no change).
+// 4 trees of 64 over 32768 keys, 32 heads over 8: 205 - 210 us a call, 0.65 PFLOP/s; matrix units busy 30 % of the time, vector units 53, waves wait for 43 % of
+// theirs, no LDS conflicts (workgroups of half the rows 215 for 212 us, over elements 136 for 139).
 #include "lm_tree.h"
 
 namespace lm {
