@@ -652,7 +652,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs p, int rows, i
     f32x4 v[8];
     auto load = [&](int s1) {
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {      // (of this round's: the next one's would be read twice, and zero times an infinity is NaN)
+      for (int s = 0; s < 8; ++s) {      // (those behind a row's lanes come with the next pass; here they would count as zero times theirs, NaN of an infinity)
         const int at = s1 + s * waves;
         v[s] = at < min(LR, parts - s0) ? *(const f32x4*)(p.part + (at0 + (s0 + at) * step) * DV + 4 * l) : zero4();
       }
